@@ -457,6 +457,55 @@ RIBN_B200_API int ribn_b200_attention_noalloc(int32_t device, void* stream, cons
                                               int32_t kv_heads, int32_t head_dim, int32_t window,
                                               float* out, char* error, size_t error_capacity);
 
+/* ---- KV cache held in 4 bits (device pointers, caller's stream) ------------ */
+/* No counterpart in the reference, whose cache is F16.  The arena is `[pages][kv_heads][18 * head_dim]` bytes (16-byte
+ * aligned, 16 tokens a page, head_dim 64, 128 or 256): per value 4 bits of code and, per 32 neighbouring dimensions of a token's
+ * head, a binary16 scale, 4.5 bits together.  A value is scale x (code - 8), exact in binary16.  The byte order is the
+ * kernels' own; a zeroed arena holds zeros.  Every pointer is a DEVICE pointer, work is enqueued on `stream` (a cudaStream_t)
+ * with `device` current (the caller's current device is restored), nothing is allocated and nothing waits, so the calls may be
+ * captured into a graph.  Refusals return RIBN_B200_ERROR with a message in ribn_b200_op_last_error and enqueue nothing.
+ * `type` is that of the rows: RIBN_B200_KVQ4_F32, _F16 or _BF16. */
+enum { RIBN_B200_KVQ4_F32 = 0, RIBN_B200_KVQ4_F16 = 1, RIBN_B200_KVQ4_BF16 = 2 };
+/* Quantises rows k, v `[rows][kv_heads][head_dim]` (`k_stride`, `v_stride`: values from one row to the next) into the arena at
+ * `slots[row]` = page * 16 + token.  Per 32 dimensions: scale = x / -8 for the value x of largest magnitude (of several the
+ * first), as binary16 with seven significant bits and at most 896 in magnitude; code = floor(value / scale + 1/2) + 8 in 0..15.
+ * NaN counts as zero; magnitudes over 7,168 come back as less.  A row whose slot lies outside of the arena (a padding row's -1) is
+ * not written.  The slots of one call are distinct: two rows of one slot leave a mixture of both in it. */
+RIBN_B200_API int ribn_b200_kvq4_append(int32_t device, void* stream, void* cache, int64_t pages, int32_t kv_heads, int32_t head_dim,
+                                        int32_t type, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                                        const int32_t* slots, int64_t rows);
+/* The cached values at `slots[row]` as rows k, v `[rows][kv_heads][head_dim]` (contiguous, 16-byte aligned); zeros where a slot
+ * lies outside of the arena.  Slots may repeat. */
+RIBN_B200_API int ribn_b200_kvq4_read(int32_t device, void* stream, const void* cache, int64_t pages, int32_t kv_heads, int32_t head_dim,
+                                      int32_t type, const int32_t* slots, int64_t rows, void* k, void* v);
+/* Causal attention over the cache, grouped queries: softmax(scale x q K^T) V.  Rows [cu_rows[s], cu_rows[s + 1]) of q
+ * `[rows][q_heads][head_dim]` are the last ones of sequence s, whose `lengths[s]` keys (the rows' own among them) lie at
+ * the pages page_tables[s * table_stride ..]: row i of n is at position lengths[s] - n + i and sees the keys up to its own, with
+ * window > 0 the last `window` of those.  A row that sees no key (its position is negative) gets zeros; rows of q that no
+ * sequence has are left alone in `out`; a page number outside of the arena hides its keys.  `max_rows` bounds the rows of
+ * a sequence (later ones are left alone); `max_keys` sets how the work is split, results are right for any.  `scale` 0 is
+ * 1 / sqrt(head_dim).  `q_stride`, `out_stride`: values from one row to the next.  `workspace` (16-byte aligned, what
+ * ribn_b200_kvq4_workspace asks for) is scratch of this call: calls that may overlap on the GPU, or graphs that may replay
+ * at once, need one each. */
+typedef struct {
+    const void* cache;
+    int64_t pages;
+    const void* q;
+    void* out;
+    const int32_t* page_tables;
+    const int32_t* lengths;   /* [sequences] */
+    const int32_t* cu_rows;   /* [sequences + 1], ascending from 0 on */
+    void* workspace;
+    size_t workspace_bytes;
+    int64_t q_stride, out_stride, table_stride;
+    int32_t type, q_heads, kv_heads, head_dim;
+    int32_t pages_per_sequence, sequences, rows, max_rows, max_keys, window;
+    float scale;
+    int32_t reserved;
+} ribn_b200_kvq4_attention_args;
+RIBN_B200_API size_t ribn_b200_kvq4_workspace(const ribn_b200_kvq4_attention_args* args);
+RIBN_B200_API int ribn_b200_kvq4_attention(int32_t device, void* stream, const ribn_b200_kvq4_attention_args* args);
+
 /* Host-side tile-major repack used by finalize (no device work): writes the
  * packed form of raw GGUF rows and returns its size; `out` may be NULL to
  * query the size.  No reference counterpart: the reference uploads GGUF bytes

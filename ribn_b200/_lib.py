@@ -13,6 +13,7 @@ ROW_READY, ROW_DEFERRED, ROW_REJECTED = 0, 1, 2
 INJECT_ALLOC_REFUSAL, INJECT_ERROR_WORD, INJECT_BAD_ROW = 1, 2, 3
 PREFILL, DECODE = 0, 1
 SCHEME_Q8_0, SCHEME_Q4_K_M = 0, 1
+KVQ4_F32, KVQ4_F16, KVQ4_BF16 = 0, 1, 2
 FLAG_KEEP_LOGITS, FLAG_REFERENCE_KERNELS, FLAG_NO_GRAPH, FLAG_NO_TCGEN05, FLAG_KV_ON_DEMAND = 1, 2, 4, 8, 16
 FLAG_OPERAND_CACHE = 32
 
@@ -56,6 +57,14 @@ class NcclId(C.Structure):
 class CompletionC(C.Structure):
     _fields_ = [("sequence", C.c_uint64), ("prefix", C.c_uint32), ("n_tokens", C.c_uint32),
                 ("token", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class KvQ4AttentionArgs(C.Structure):
+    _fields_ = [("cache", C.c_void_p), ("pages", C.c_int64)] + \
+        [(n, C.c_void_p) for n in ("q", "out", "page_tables", "lengths", "cu_rows", "workspace")] + [("workspace_bytes", C.c_size_t)] + \
+        [(n, C.c_int64) for n in ("q_stride", "out_stride", "table_stride")] + \
+        [(n, C.c_int32) for n in ("type", "q_heads", "kv_heads", "head_dim", "pages_per_sequence", "sequences", "rows", "max_rows",
+                                  "max_keys", "window")] + [("scale", C.c_float), ("reserved", C.c_int32)]
 
 
 _P = C.c_void_p
@@ -115,6 +124,11 @@ SIGNATURES = {
                                               _P, _P]),
     "ribn_b200_attention_noalloc": (C.c_int, [C.c_int32, _P, _P, _P, _P, _P, _P, C.c_int32, C.c_int32, C.c_int32,
                                               C.c_int32, C.c_int32, C.c_int32, _P, C.c_char_p, C.c_size_t]),
+    "ribn_b200_kvq4_append": (C.c_int, [C.c_int32, _P, _P, C.c_int64, C.c_int32, C.c_int32, C.c_int32, _P, C.c_int64, _P, C.c_int64, _P,
+                                        C.c_int64]),
+    "ribn_b200_kvq4_read": (C.c_int, [C.c_int32, _P, _P, C.c_int64, C.c_int32, C.c_int32, C.c_int32, _P, C.c_int64, _P, _P]),
+    "ribn_b200_kvq4_workspace": (C.c_size_t, [C.POINTER(KvQ4AttentionArgs)]),
+    "ribn_b200_kvq4_attention": (C.c_int, [C.c_int32, _P, C.POINTER(KvQ4AttentionArgs)]),
     "ribn_b200_debug_step_deal": (C.c_int, [C.c_int32, C.c_int64, C.c_int64, C.c_int32, _P, C.c_size_t, C.POINTER(C.c_size_t),
                                             C.POINTER(C.c_size_t), C.POINTER(C.c_size_t)]),
     "ribn_b200_debug_step_operand": (C.c_int, [C.c_int32, C.c_int32, _P, _P, _P, C.c_int32, C.c_int32, _P, C.c_size_t, C.POINTER(C.c_size_t)]),

@@ -1,0 +1,70 @@
+// The KV cache held in 4 bits: layout, arguments of its launchers, and what its kernels share.
+//
+// The arena is [pages][kv_heads][18 head_dim] bytes, 16 tokens a page: a page of one head is one contiguous record
+//   K codes, 8 head_dim bytes   [sub][token j][t][w][4 bytes]       nibble i of a word: dimension 32 G + 8 t + i
+//   V codes, 8 head_dim bytes   [sub][c][g][t][w][e][2 bytes]       nibble i of a half word: dimension 32 G + 8 i + g, j = 8 c + 2 t + e
+//   K scales, head_dim bytes    [j][G] binary16
+//   V scales, head_dim bytes    [c][t][G][e] binary16
+// with G = 4 sub + w the group of 32 dimensions (a head of 64 has two: w < 2).  A value is scale x (code - 8).  A scale has seven
+// significant bits, so the value (four more) and 72 x scale (four more) are binary16 numbers, without any rounding.
+//
+// The order is the matrix instructions': of a K page a lane (g = lane / 4, t = lane % 4) reads 16 bytes of keys g and g + 8, of a
+// V page 16 bytes of key pairs 2 t and 8 + 2 t, and masks and shifts turn the words into the operands of m16n8k16 with the keys
+// (K) or the dimensions (V) as rows.  A byte belongs to one token, so writing a token's row reads nothing.
+#pragma once
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "gemv.cuh"
+
+namespace ribn {
+
+constexpr int kQ4Page = 16;            // tokens per page
+constexpr int kQ4MaxGroup = 16;        // query heads per kv head
+__host__ __device__ constexpr int q4_record(int head_dim) { return 18 * head_dim; }
+
+enum Q4Type : int { kQ4F32 = 0, kQ4F16 = 1, kQ4BF16 = 2 };
+
+struct KvQ4Rows {
+    unsigned char* cache;
+    long long pages;
+    int kv_heads, head_dim, type;
+    const void* k;                     // [rows][kv_heads][head_dim]; written by a read
+    const void* v;
+    long long k_stride, v_stride;      // values between rows
+    const int32_t* slots;              // page * 16 + token; outside of the arena: the row is skipped (append) or zero (read)
+    long long rows;
+};
+cudaError_t launch_kvq4_append(cudaStream_t stream, const KvQ4Rows& a);
+cudaError_t launch_kvq4_read(cudaStream_t stream, const KvQ4Rows& a);
+
+struct KvQ4Attention {
+    const unsigned char* cache;
+    long long pages;
+    int q_heads, kv_heads, head_dim, type;
+    const void* q;                     // [rows][q_heads][head_dim]
+    long long q_stride, out_stride;    // values between rows
+    void* out;
+    const int32_t* page_tables;        // [sequences][table_stride]
+    int pages_per_sequence;
+    long long table_stride;
+    const int32_t* lengths;            // [sequences] keys, the new rows' among them
+    const int32_t* cu_rows;            // [sequences + 1]
+    int sequences, rows, max_rows, max_keys, window;
+    float scale;                       // of the scores
+    float* partial;                    // spans' sums
+    size_t partial_bytes;
+    // set by the launcher
+    int max_spans, span_pages, span_cols, col_blocks, vector_q, vector_out;
+};
+// Floats of partial sums that launch_kvq4_attention may use.
+size_t kvq4_partial_floats(const KvQ4Attention& a);
+cudaError_t launch_kvq4_attention(cudaStream_t stream, KvQ4Attention a);
+
+int kvq4_sm_count();
+
+// Sets the calling thread's operator diagnostic (ops_api.cu); returns RIBN_B200_ERROR.
+int op_error(const char* what, cudaError_t e);
+
+}  // namespace ribn

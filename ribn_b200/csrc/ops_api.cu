@@ -17,6 +17,7 @@
 #include "blocks.cuh"
 #include "gemv.cuh"
 #include "kernels.cuh"
+#include "kvq4.cuh"
 #include "step_operand.cuh"
 
 using namespace ribn;
@@ -89,6 +90,14 @@ __global__ void quotient_kernel(const float* x, const float* den, size_t n, floa
 }
 
 }  // namespace
+
+namespace ribn {
+int op_error(const char* what, cudaError_t e) {
+    if (e != cudaSuccess) return op_fail(what, e);
+    g_op_error = what;
+    return RIBN_B200_ERROR;
+}
+}  // namespace ribn
 
 extern "C" {
 

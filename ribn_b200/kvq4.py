@@ -1,0 +1,129 @@
+"""The KV cache held in 4 bits: rows written into a paged arena, values read back, and attention over it.
+
+A serving program keeps one arena per layer (:func:`empty_cache`, a torch uint8 tensor ``[pages][kv_heads][18 * head_dim]``,
+16 tokens a page, 4.5 bits per value) beside its page tables.  Tensors lie on one CUDA device; every call is enqueued on that
+device's current stream, allocates at most its result and its scratch through torch, and may be captured into a graph.  These
+are the calls of ``include/ribn_b200.h`` (``ribn_b200_kvq4_*``), where the format and the rules are written down; there is no
+CPU path.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from ._lib import KVQ4_BF16, KVQ4_F16, KVQ4_F32, OK, KvQ4AttentionArgs, lib
+
+PAGE_TOKENS = 16
+_TYPES = {torch.float32: KVQ4_F32, torch.float16: KVQ4_F16, torch.bfloat16: KVQ4_BF16}
+
+
+def empty_cache(pages: int, kv_heads: int, head_dim: int, device="cuda") -> torch.Tensor:
+    """An arena of `pages` 16-token pages, all values zero."""
+    if head_dim not in (64, 128, 256) or pages <= 0 or kv_heads <= 0:
+        raise ValueError("an arena has pages, kv heads and a head_dim of 64, 128 or 256")
+    return torch.zeros((pages, kv_heads, 18 * head_dim), dtype=torch.uint8, device=device)
+
+
+def _refuse(what: str):
+    buf = C.create_string_buffer(1024)
+    lib().ribn_b200_op_last_error(buf, len(buf))
+    raise RuntimeError(f"ribn_b200 {what} failed: {buf.value.decode(errors='replace')}")
+
+
+def _arena(cache: torch.Tensor):
+    if cache.dtype is not torch.uint8 or cache.dim() != 3 or not cache.is_contiguous() or not cache.is_cuda or cache.shape[2] % 18:
+        raise ValueError("cache must be a contiguous uint8 CUDA tensor [pages][kv_heads][18 * head_dim]")
+    pages, kv_heads, record = cache.shape
+    return pages, kv_heads, record // 18, cache.device
+
+
+def _rows(name: str, x: torch.Tensor, heads: int, head_dim: int, device, rows: int | None = None, dtype=None):
+    """A [rows][heads][head_dim] tensor whose rows are whole; the values from one row to the next."""
+    shape, stride = x.shape, x.stride()
+    if len(shape) != 3 or shape[1] != heads or shape[2] != head_dim or (rows is not None and shape[0] != rows):
+        raise ValueError(f"{name} must be [{'rows' if rows is None else rows}][{heads}][{head_dim}]: got {list(shape)}")
+    if x.device != device or x.dtype not in _TYPES or (dtype is not None and x.dtype is not dtype):
+        raise ValueError(f"{name} must be float32, float16 or bfloat16, as its fellows are, on {device}: got {x.dtype} on {x.device}")
+    if shape[0] and (stride[2] != 1 or (heads > 1 and stride[1] != head_dim)):
+        raise ValueError(f"{name}: the heads of a row must lie side by side")
+    if shape[0] > 1 and stride[0] < heads * head_dim:
+        raise ValueError(f"{name}: rows overlap")
+    return stride[0]
+
+
+def _ints(name: str, x: torch.Tensor, dims: int, device):
+    if x.dtype is not torch.int32 or x.dim() != dims or x.device != device or (x.numel() and x.stride(dims - 1) != 1):
+        raise ValueError(f"{name} must be a {dims}-dimensional int32 tensor on {device}, its last dimension contiguous")
+    return x.data_ptr()
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def append(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+    """Quantises rows k, v [rows][kv_heads][head_dim] into the arena at slots[row] = page * 16 + token.  A row with a slot outside
+    of the arena (-1: padding) is not written.  The slots of one call are distinct.  NaN counts as zero, magnitudes over 7,168
+    saturate."""
+    pages, kv_heads, head_dim, device = _arena(cache)
+    k_stride = _rows("k", k, kv_heads, head_dim, device)
+    rows = k.shape[0]
+    v_stride = _rows("v", v, kv_heads, head_dim, device, rows, k.dtype)
+    at = _ints("slots", slots, 1, device)
+    if slots.shape[0] != rows:
+        raise ValueError("slots must name one slot per row")
+    if lib().ribn_b200_kvq4_append(device.index, _stream(device), cache.data_ptr(), pages, kv_heads, head_dim, _TYPES[k.dtype], k.data_ptr(),
+                                   k_stride, v.data_ptr(), v_stride, at, rows) != OK:
+        _refuse("kvq4_append")
+
+
+def read(cache: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = torch.float16):
+    """(k, v) [rows][kv_heads][head_dim]: the cached values at slots[row], which float16 and float32 hold exactly; zeros where a slot
+    lies outside of the arena."""
+    pages, kv_heads, head_dim, device = _arena(cache)
+    at = _ints("slots", slots, 1, device)
+    if dtype not in _TYPES:
+        raise ValueError("dtype must be float32, float16 or bfloat16")
+    rows = slots.shape[0]
+    k, v = torch.empty((2, rows, kv_heads, head_dim), dtype=dtype, device=device).unbind(0)
+    if lib().ribn_b200_kvq4_read(device.index, _stream(device), cache.data_ptr(), pages, kv_heads, head_dim, _TYPES[dtype], at, rows,
+                                 k.data_ptr(), v.data_ptr()) != OK:
+        _refuse("kvq4_read")
+    return k, v
+
+
+def attention(cache: torch.Tensor, q: torch.Tensor, page_tables: torch.Tensor, lengths: torch.Tensor, cu_rows: torch.Tensor, *,
+              max_rows: int, max_keys: int, window: int = 0, scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal grouped-query attention over the arena: rows [cu_rows[s], cu_rows[s + 1]) of q [rows][q_heads][head_dim] are the last
+    rows of sequence s, which has lengths[s] keys (these rows' own, already appended, among them) in the pages page_tables[s].
+    Row i of n sits at position lengths[s] - n + i and sees the keys up to its own, with window > 0 the last `window` of those.
+
+    Rows that see no key get zeros, rows behind the last sequence stay as they are in `out` (zeros in a new one).  `max_rows` is
+    the most rows of a sequence; `max_keys`, about the longest length, decides how the work is split and no result.
+    `scale` defaults to head_dim ** -0.5.  Returns `out`, of q's type."""
+    pages, kv_heads, head_dim, device = _arena(cache)
+    if q.dim() != 3 or q.shape[1] == 0 or q.shape[1] % kv_heads:
+        raise ValueError(f"q must be [rows][q_heads][{head_dim}], q_heads a multiple of the cache's {kv_heads}")
+    rows, q_heads, _ = q.shape
+    q_stride = _rows("q", q, q_heads, head_dim, device)
+    sequences = lengths.shape[0] if lengths.dim() == 1 else -1
+    tables, at_lengths, at_rows = _ints("page_tables", page_tables, 2, device), _ints("lengths", lengths, 1, device), _ints("cu_rows", cu_rows, 1, device)
+    if page_tables.shape[0] != sequences or cu_rows.shape[0] != sequences + 1:
+        raise ValueError("page_tables, lengths and cu_rows must have sequences, sequences and sequences + 1 rows")
+    if scale is not None and not 0.0 < abs(scale) < float("inf"):
+        raise ValueError("scale must be finite and not zero")
+    if out is None:
+        out = torch.zeros((rows, q_heads, head_dim), dtype=q.dtype, device=device)
+    out_stride = _rows("out", out, q_heads, head_dim, device, rows, q.dtype)
+    args = KvQ4AttentionArgs(cache.data_ptr(), pages, q.data_ptr(), out.data_ptr(), tables, at_lengths, at_rows, None, 0, q_stride, out_stride,
+                             page_tables.stride(0), _TYPES[q.dtype], q_heads, kv_heads, head_dim, page_tables.shape[1], sequences, rows,
+                             min(max_rows, rows), max_keys, window, scale or 0.0, 0)
+    library = lib()
+    need = library.ribn_b200_kvq4_workspace(args)
+    if need:
+        scratch = torch.empty(need, dtype=torch.uint8, device=device)
+        args.workspace, args.workspace_bytes = scratch.data_ptr(), need
+    if library.ribn_b200_kvq4_attention(device.index, _stream(device), args) != OK:
+        _refuse("kvq4_attention")
+    return out
