@@ -15,39 +15,6 @@ namespace {
 
 __device__ __forceinline__ uint32_t bits_of(__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); }
 
-template <int TYPE>
-__device__ __forceinline__ void load8(const void* base, long long at, bool vector, float (&x)[8]) {
-    if (TYPE == kQ4F32) {
-        const float* p = static_cast<const float*>(base) + at;
-        if (vector) {
-            const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = p[i];
-        }
-    } else {
-        const unsigned short* p = static_cast<const unsigned short*>(base) + at;
-        uint32_t w[4];
-        if (vector) {
-            const uint4 a = *reinterpret_cast<const uint4*>(p);
-            w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = (uint32_t)p[2 * i] | ((uint32_t)p[2 * i + 1] << 16);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (TYPE == kQ4F16) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-                x[2 * i] = f.x; x[2 * i + 1] = f.y;
-            } else {
-                x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-            }
-        }
-    }
-}
-
 // Eight values that binary16 holds exactly
 template <int TYPE>
 __device__ __forceinline__ void store8(void* base, long long at, const __half2 (&x)[4]) {
@@ -137,7 +104,7 @@ __global__ void __launch_bounds__(256) kvq4_append_kernel(const KvQ4Rows a, cons
     float x[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-    if (live) load8<TYPE>(at.which ? a.v : a.k, at.row * (at.which ? a.v_stride : a.k_stride) + (long long)at.head * a.head_dim + at.p * 8, vector, x);
+    if (live) q4_load8(at.which ? a.v : a.k, at.row * (at.which ? a.v_stride : a.k_stride) + (long long)at.head * a.head_dim + at.p * 8, TYPE, vector, x);
     float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {

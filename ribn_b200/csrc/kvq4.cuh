@@ -57,12 +57,49 @@ struct KvQ4Attention {
     size_t partial_bytes;
     // set by the launcher
     int max_spans, span_pages, span_cols, col_blocks, vector_q, vector_out;
+    int tile_above;                    // a sequence with more query rows (rows x heads of a group) than this takes the tile kernel
 };
 // Floats of partial sums that launch_kvq4_attention may use.
 size_t kvq4_partial_floats(const KvQ4Attention& a);
 cudaError_t launch_kvq4_attention(cudaStream_t stream, KvQ4Attention a);
 
+// The sequences with more than `tile_above` query rows (kvq4_tile.cu; heads of 64 and 128).
+cudaError_t launch_kvq4_tiles(cudaStream_t stream, const KvQ4Attention& a);
+
 int kvq4_sm_count();
+
+// Eight neighbouring values of a row as F32
+__device__ __forceinline__ void q4_load8(const void* base, long long at, int type, bool vector, float (&x)[8]) {
+    if (type == kQ4F32) {
+        const float* p = static_cast<const float*>(base) + at;
+        if (vector) {
+            const float4 u = *reinterpret_cast<const float4*>(p), v = *reinterpret_cast<const float4*>(p + 4);
+            x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = p[i];
+        }
+        return;
+    }
+    const unsigned short* p = static_cast<const unsigned short*>(base) + at;
+    uint32_t w[4];
+    if (vector) {
+        const uint4 u = *reinterpret_cast<const uint4*>(p);
+        w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = (uint32_t)p[2 * i] | ((uint32_t)p[2 * i + 1] << 16);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (type == kQ4F16) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            x[2 * i] = f.x; x[2 * i + 1] = f.y;
+        } else {
+            x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+}
 
 // Sets the calling thread's operator diagnostic (ops_api.cu); returns RIBN_B200_ERROR.
 int op_error(const char* what, cudaError_t e);

@@ -69,38 +69,6 @@ __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
     return v;
 }
 
-// Eight neighbouring values of a query row
-__device__ __forceinline__ void load_query8(const KvQ4Attention& a, long long at, float (&x)[8]) {
-    if (a.type == kQ4F32) {
-        const float* p = static_cast<const float*>(a.q) + at;
-        if (a.vector_q) {
-            const float4 u = *reinterpret_cast<const float4*>(p), v = *reinterpret_cast<const float4*>(p + 4);
-            x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = p[i];
-        }
-        return;
-    }
-    const unsigned short* p = static_cast<const unsigned short*>(a.q) + at;
-    uint32_t w[4];
-    if (a.vector_q) {
-        const uint4 u = *reinterpret_cast<const uint4*>(p);
-        w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = (uint32_t)p[2 * i] | ((uint32_t)p[2 * i + 1] << 16);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (a.type == kQ4F16) {
-            const float2 f = __half22float2(half2_of(w[i]));
-            x[2 * i] = f.x; x[2 * i + 1] = f.y;
-        } else {
-            x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
-    }
-}
 __device__ __forceinline__ void store_value(const KvQ4Attention& a, long long at, float x) {
     if (a.type == kQ4F32) static_cast<float*>(a.out)[at] = x;
     else if (a.type == kQ4F16) static_cast<__half*>(a.out)[at] = __float2half_rn(x);
@@ -120,7 +88,7 @@ __device__ __forceinline__ Block block_of(const KvQ4Attention& a, int s, int cb)
     b.n = min(a.cu_rows[s + 1], a.rows) - b.row0;
     const int length = min(max(a.lengths[s], 0), a.pages_per_sequence * kQ4Page);
     b.base = length - b.n;
-    b.cols = max(0, min(a.span_cols, b.n * group - cb * a.span_cols));
+    b.cols = (long long)b.n * group > a.tile_above ? 0 : max(0, min(a.span_cols, b.n * group - cb * a.span_cols));   // 0: the tile kernel's
     b.first_row = cb * a.span_cols / group;
     b.last_row = (cb * a.span_cols + b.cols - 1) / group;
     b.high = max(0, b.base + b.last_row + 1);
@@ -197,7 +165,7 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 && NT == 1 ? (PAIR ? 3 
         for (int G = 0; G < NG; ++G) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[G][i] = 0.0f;
-            if (have) load_query8(a, (b.row0 + flat / group) * a.q_stride + (long long)(kvh * group + flat % group) * HD + 32 * G + 8 * t, x[G]);
+            if (have) q4_load8(a.q, (b.row0 + flat / group) * a.q_stride + (long long)(kvh * group + flat % group) * HD + 32 * G + 8 * t, a.type, a.vector_q, x[G]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[G][i]));
         }
@@ -382,12 +350,18 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 && NT == 1 ? (PAIR ? 3 
                     const uint32_t upper[4] = {value(w0[w] >> 4, a0, b0), value(w0[w] >> 8, a0, b0), value(w1[w] >> 4, a1, b1), value(w1[w] >> 8, a1, b1)};
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        if (PAIR) {
-                            mma(o[nt][2 * G], lower, pl[PAIR ? nt : 0][0], pl[PAIR ? nt : 0][1], o[nt][2 * G]);
-                            mma(o[nt][2 * G + 1], upper, pl[PAIR ? nt : 0][0], pl[PAIR ? nt : 0][1], o[nt][2 * G + 1]);
+                        if (PAIR) {   // a page's sum by itself: the instruction cuts at the last bit of what it adds to
+                            float lo[4] = {0.0f, 0.0f, 0.0f, 0.0f}, up[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            mma(lo, lower, pl[PAIR ? nt : 0][0], pl[PAIR ? nt : 0][1], lo);
+                            mma(up, upper, pl[PAIR ? nt : 0][0], pl[PAIR ? nt : 0][1], up);
+                            mma(lo, lower, ph[nt][0], ph[nt][1], lo);
+                            mma(up, upper, ph[nt][0], ph[nt][1], up);
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) { o[nt][2 * G][u] += lo[u]; o[nt][2 * G + 1][u] += up[u]; }
+                        } else {
+                            mma(o[nt][2 * G], lower, ph[nt][0], ph[nt][1], o[nt][2 * G]);
+                            mma(o[nt][2 * G + 1], upper, ph[nt][0], ph[nt][1], o[nt][2 * G + 1]);
                         }
-                        mma(o[nt][2 * G], lower, ph[nt][0], ph[nt][1], o[nt][2 * G]);
-                        mma(o[nt][2 * G + 1], upper, ph[nt][0], ph[nt][1], o[nt][2 * G + 1]);
                     }
                 }
             }
@@ -467,7 +441,7 @@ __global__ void __launch_bounds__(kWarps * 32) kvq4_merge_kernel(const KvQ4Atten
     const int flat = (row - a.cu_rows[s]) * group + qh % group;
     if (flat / a.span_cols >= a.col_blocks) return;   // more rows than the call said
     const Block b = block_of(a, s, flat / a.span_cols);
-    if (b.spans <= 1) return;   // written by the span kernel
+    if (b.cols <= 0 || b.spans <= 1) return;   // written by the tile or the span kernel
     const float* pp = a.partial + ((long long)row * a.q_heads + qh) * a.max_spans * REC;
     float top = -INFINITY;
     for (int i = lane; i < b.spans; i += 32) top = fmaxf(top, __ldcg(pp + (long long)i * REC + HD));
@@ -510,7 +484,9 @@ bool aligned16(const void* p, long long stride, int size) { return (reinterpret_
 
 // How a launch is split: columns per CTA and spans.
 void plan_spans(KvQ4Attention& a) {
-    const int group = a.q_heads / a.kv_heads, cols = std::min(a.max_rows, a.rows) * group;
+    const int group = a.q_heads / a.kv_heads;
+    a.tile_above = a.head_dim == 256 ? 0x7fffffff : 32;
+    const int cols = (int)std::min<long long>((long long)std::min(a.max_rows, a.rows) * group, a.tile_above);
     // 16 columns share a page's conversion; with heads of 256 their sums do not fit in the registers (1,080 bytes of spills)
     a.span_cols = cols <= 8 || a.head_dim == 256 ? 8 : 16;
     a.col_blocks = (cols + a.span_cols - 1) / a.span_cols;
@@ -597,6 +573,10 @@ cudaError_t launch_kvq4_attention(cudaStream_t stream, KvQ4Attention a) {
     const int size = a.type == kQ4F32 ? 4 : 2;
     a.vector_q = aligned16(a.q, a.q_stride, size);
     a.vector_out = aligned16(a.out, a.out_stride, size);
+    if ((long long)a.max_rows * (a.q_heads / a.kv_heads) > a.tile_above) {
+        const cudaError_t e = launch_kvq4_tiles(stream, a);
+        if (e != cudaSuccess) return e;
+    }
     switch (a.head_dim) {
         case 64: return launch_hd<64>(stream, a);
         case 128: return launch_hd<128>(stream, a);

@@ -191,15 +191,32 @@ def test_long_ranges_are_split_and_joined(kvq4, d, keys, type_name):
     assert torch.isfinite(out).all()
 
 
-def test_pages_outside_of_the_arena_hide_their_keys(kvq4):
+@pytest.mark.parametrize("type_name", TYPES)
+@pytest.mark.parametrize("counts,lengths,window,q_heads,kv_heads,d", [
+    ([130], [130], 0, 4, 2, 128), ([64], [64], 0, 2, 1, 64), ([300], [1100], 0, 4, 1, 128), ([70, 1, 33, 0, 200], [700, 650, 33, 9, 260], 0, 4, 2, 64),
+    ([150], [900], 100, 3, 1, 128), ([257], [300], 1, 2, 1, 64), ([150, 2], [100, 1], 0, 16, 1, 128)])
+def test_prompt_chunks_beside_single_rows(kvq4, counts, lengths, window, q_heads, kv_heads, d, type_name):
+    """Chunks alone, behind a prefix, over several blocks of rows and keys, longer than their sequence (the first rows see nothing), with
+    windows that begin inside a block, and single rows and an empty sequence among them."""
+    dtype, unit = TYPES[type_name]
+    rng = np.random.default_rng(sum(counts))
+    cu = [0, *np.cumsum(counts).tolist()]
+    pages = sum((n + 15) // 16 for n in lengths) + 2
+    cache, arena = _filled(kvq4, rng, pages, kv_heads, d)
+    q = _rows(rng, cu[-1] + 3, q_heads, d, dtype, 1.5)
+    _call(kvq4, cache, arena, q, _tables(rng, pages, lengths), lengths, cu, max(counts), window=window, unit=unit)
+
+
+@pytest.mark.parametrize("rows", [1, 90])
+def test_pages_outside_of_the_arena_hide_their_keys(kvq4, rows):
     rng = np.random.default_rng(8)
     cache, arena = _filled(kvq4, rng, 12, 2, 128)
     lengths = [150, 40]
     tables = _tables(rng, 12, [150, 32])
     tables[0, 3], tables[0, 9], tables[1, :] = -1, 12, 1 << 30
-    q = _rows(rng, 2, 8, 128, torch.float16)
-    out = _call(kvq4, cache, arena, q, tables, lengths, [0, 1, 2], 1, unit=2.0 ** -11)
-    assert not out[1].any()   # every page hidden
+    q = _rows(rng, rows + 1, 8, 128, torch.float16)
+    out = _call(kvq4, cache, arena, q, tables, lengths, [0, rows, rows + 1], rows, unit=2.0 ** -11)
+    assert not out[rows].any()   # every page hidden
 
 
 @pytest.mark.parametrize("rows", [1, 20])
