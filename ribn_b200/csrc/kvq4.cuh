@@ -57,10 +57,12 @@ struct KvQ4Attention {
     size_t partial_bytes;
     // set by the launcher
     int max_spans, span_pages, span_cols, col_blocks, vector_q, vector_out;
+    unsigned char* scratch;            // operands of the tile kernel's key tiles, [tile][kv_head][512 head_dim bytes]
+    int scratch_tiles;                 // how many tiles there is room for
     int tile_above;                    // a sequence with more query rows (rows x heads of a group) than this takes the tile kernel
 };
-// Floats of partial sums that launch_kvq4_attention may use.
-size_t kvq4_partial_floats(const KvQ4Attention& a);
+// Bytes of scratch that launch_kvq4_attention can use; it works with less than the tile kernel's part, not with less than the sums.
+size_t kvq4_workspace_bytes(const KvQ4Attention& a);
 cudaError_t launch_kvq4_attention(cudaStream_t stream, KvQ4Attention a);
 
 // The sequences with more than `tile_above` query rows (kvq4_tile.cu; heads of 64 and 128).

@@ -104,7 +104,7 @@ int ribn_b200_kvq4_read(int32_t device, void* stream, const void* cache, int64_t
 
 size_t ribn_b200_kvq4_workspace(const ribn_b200_kvq4_attention_args* args) {
     if (args == nullptr || bad_attention(*args) != nullptr || args->rows == 0 || args->sequences == 0 || args->max_rows == 0) return 0;
-    return kvq4_partial_floats(attention_of(*args)) * sizeof(float);
+    return kvq4_workspace_bytes(attention_of(*args));
 }
 
 int ribn_b200_kvq4_attention(int32_t device, void* stream, const ribn_b200_kvq4_attention_args* args) {

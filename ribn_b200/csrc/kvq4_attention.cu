@@ -560,16 +560,38 @@ int kvq4_sm_count() {
     return counts[dev];
 }
 
-size_t kvq4_partial_floats(const KvQ4Attention& args) {
+namespace {
+
+// Bytes of the spans' sums, and behind them room for the tile kernel's operands: at most kScratchMost, or what the sequences with
+// enough rows can need.
+constexpr size_t kScratchMost = 512u << 20;
+size_t partial_bytes(const KvQ4Attention& a) {
+    const size_t n = a.max_spans > 1 ? (size_t)a.rows * a.q_heads * a.max_spans * (a.head_dim + 2) * sizeof(float) : 0;
+    return (n + 255) / 256 * 256;
+}
+int wanted_tiles(const KvQ4Attention& a) {
+    const long long flats = (long long)a.rows * (a.q_heads / a.kv_heads);
+    if ((long long)std::min(a.max_rows, a.rows) * (a.q_heads / a.kv_heads) <= a.tile_above) return 0;
+    const long long keys = a.window > 0 ? std::min<long long>(a.max_keys, (long long)a.window + a.max_rows) : a.max_keys;
+    const long long tiles = std::min<long long>(a.sequences, flats / (a.tile_above + 1)) * (keys / 128 + 2), room = (long long)(kScratchMost / ((size_t)512 * a.head_dim * a.kv_heads));
+    return (int)std::min(tiles, room);
+}
+
+}  // namespace
+
+size_t kvq4_workspace_bytes(const KvQ4Attention& args) {
     KvQ4Attention a = args;
     plan_spans(a);
-    return a.max_spans > 1 ? (size_t)a.rows * a.q_heads * a.max_spans * (a.head_dim + 2) : 0;
+    return partial_bytes(a) + (size_t)wanted_tiles(a) * 512 * a.head_dim * a.kv_heads;
 }
 
 cudaError_t launch_kvq4_attention(cudaStream_t stream, KvQ4Attention a) {
     if (a.rows <= 0 || a.sequences <= 0) return cudaSuccess;
     plan_spans(a);
-    if (a.max_spans > 1 && a.partial_bytes < (size_t)a.rows * a.q_heads * a.max_spans * (a.head_dim + 2) * sizeof(float)) return cudaErrorInvalidValue;
+    const size_t sums = partial_bytes(a);
+    if (a.partial_bytes < sums) return cudaErrorInvalidValue;
+    a.scratch = reinterpret_cast<unsigned char*>(a.partial) + sums;
+    a.scratch_tiles = (int)std::min<size_t>((size_t)wanted_tiles(a), (a.partial_bytes - sums) / ((size_t)512 * a.head_dim * a.kv_heads));
     const int size = a.type == kQ4F32 ? 4 : 2;
     a.vector_q = aligned16(a.q, a.q_stride, size);
     a.vector_out = aligned16(a.out, a.out_stride, size);
