@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(256) kvq4_append_kernel(const KvQ4Rows a, cons
     float x[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-    if (live) q4_load8(at.which ? a.v : a.k, at.row * (at.which ? a.v_stride : a.k_stride) + (long long)at.head * a.head_dim + at.p * 8, TYPE, vector, x);
+    if (live) q4_load8<TYPE == kQ4F32>(at.which ? a.v : a.k, at.row * (at.which ? a.v_stride : a.k_stride) + (long long)at.head * a.head_dim + at.p * 8, TYPE, vector, x);
     float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {

@@ -53,10 +53,11 @@ struct KvQ4Attention {
     const int32_t* cu_rows;            // [sequences + 1]
     int sequences, rows, max_rows, max_keys, window;
     float scale;                       // of the scores
-    float* partial;                    // spans' sums
+    float* partial;                    // scratch of partial_bytes: the runs' sums and the operands below
     size_t partial_bytes;
     // set by the launcher
-    int max_spans, span_pages, span_cols, col_blocks, vector_q, vector_out;
+    int grid, least_pages, max_spans, span_cols, col_blocks, merge_cols, vector_q, vector_out;
+    long long* prefix;                 // pages of the span kernel's list before each sequence, and of all
     unsigned char* scratch;            // operands of the tile kernel's key tiles, [tile][kv_head][512 head_dim bytes]
     int scratch_tiles;                 // how many tiles there is room for
     int tile_above;                    // a sequence with more query rows (rows x heads of a group) than this takes the tile kernel
@@ -70,40 +71,48 @@ cudaError_t launch_kvq4_tiles(cudaStream_t stream, const KvQ4Attention& a);
 
 int kvq4_sm_count();
 
-// Eight neighbouring values of a row as F32
-__device__ __forceinline__ void q4_load8(const void* base, long long at, int type, bool vector, float (&x)[8]) {
-    if (type == kQ4F32) {
-        const float* p = static_cast<const float*>(base) + at;
-        if (vector) {
-            const float4 u = *reinterpret_cast<const float4*>(p), v = *reinterpret_cast<const float4*>(p + 4);
-            x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = p[i];
-        }
-        return;
-    }
-    const unsigned short* p = static_cast<const unsigned short*>(base) + at;
-    uint32_t w[4];
+// Sets the calling thread's operator diagnostic (ops_api.cu); returns RIBN_B200_ERROR.
+int op_error(const char* what, cudaError_t e);
+
+// Eight neighbouring values of a row as they lie (F32: eight words, else four) ..
+template <int WORDS>
+__device__ __forceinline__ void q4_load_raw(const void* base, long long at, bool vector, uint32_t (&w)[WORDS]) {
     if (vector) {
-        const uint4 u = *reinterpret_cast<const uint4*>(p);
-        w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(base) + at * (WORDS / 2));
+#pragma unroll
+        for (int i = 0; i < WORDS / 4; ++i) {
+            const uint4 u = p[i];
+            w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
+        }
+    } else if (WORDS == 8) {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) w[i] = static_cast<const uint32_t*>(base)[at + i];
     } else {
+        const unsigned short* p = static_cast<const unsigned short*>(base) + at;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = (uint32_t)p[2 * i] | ((uint32_t)p[2 * i + 1] << 16);
+        for (int i = 0; i < WORDS; ++i) w[i] = (uint32_t)p[2 * i] | ((uint32_t)p[2 * i + 1] << 16);
     }
+}
+// .. and as F32
+template <int WORDS>
+__device__ __forceinline__ void q4_values(const uint32_t (&w)[WORDS], int type, float (&x)[8]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (type == kQ4F16) {
+    for (int i = 0; i < WORDS; ++i) {
+        if (WORDS == 8) {
+            x[i] = __uint_as_float(w[i]);
+        } else if (type == kQ4F16) {
             const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-            x[2 * i] = f.x; x[2 * i + 1] = f.y;
+            x[(2 * i) & 7] = f.x; x[(2 * i + 1) & 7] = f.y;
         } else {
-            x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            x[(2 * i) & 7] = __uint_as_float(w[i] << 16); x[(2 * i + 1) & 7] = __uint_as_float(w[i] & 0xffff0000u);
         }
     }
 }
-
-// Sets the calling thread's operator diagnostic (ops_api.cu); returns RIBN_B200_ERROR.
-int op_error(const char* what, cudaError_t e);
+template <bool WIDE>
+__device__ __forceinline__ void q4_load8(const void* base, long long at, int type, bool vector, float (&x)[8]) {
+    uint32_t w[WIDE ? 8 : 4];
+    q4_load_raw(base, at, vector, w);
+    q4_values(w, type, x);
+}
 
 }  // namespace ribn

@@ -1,17 +1,21 @@
 // Attention over the 4-bit paged KV cache (kvq4.cuh): a few query rows per sequence against long key ranges.
 //
-// A CTA of four warps takes a span of pages of one (sequence, kv head) for a block of up to 8 or 16 columns (column = row of the
-// sequence x query head of the group); warp w takes pages w, w + 4, .. and is a pipeline of its own: page records come into its
-// ring of shared memory by asynchronous copies, kRing - 1 pages ahead.  With m16n8k16 products, per page of 16 keys:
+// The work is the list of all (sequence, kv head, block of columns) items' pages, one after the other (column = row of the sequence x
+// query head of the group, up to 8 or 16 per block); every CTA has an equal run of it, whatever the sequences' lengths, so it begins
+// and ends inside items; what it has of an item that it shares with others meets theirs in the merge kernel, in page order.  Within an
+// item's run warp w of four takes pages w, w + 4, .. and is a pipeline of its own: page records come into its ring of shared memory
+// by asynchronous copies, kRing - 1 pages ahead.  With m16n8k16 products, per page of 16 keys:
 //   S^T = K Q^T   a masked nibble is a binary16 number by itself, code x 2^-24 (or, one nibble up, 2^-20: those dimensions' queries
 //                 are held 2^-4 times), so a word of eight codes costs a shift and four masks and no conversion.  A group of 32
 //                 dimensions is summed apart, beginning with -8 x the sum of its queries, and enters the score times its scale.
 //                 Queries are scaled by a power of two per column, so that binary16 holds F16 and BF16 ones exactly.
 //   O^T = V^T P^T a nibble under the exponent of 64 is 64 + code; one fused multiply-add with the scale and -72 x scale, both exact,
 //                 gives the value.  P comes from the S^T layout by transposing 8 x 8 blocks across the warp.
-// F32 queries and their probabilities are binary16 hi + lo pairs (two products each).  Softmax in base 2; a column's reference moves
-// only when a score passes it by 2^8, and P is held 2^7 times, so that small probabilities stay normal numbers.
-// The spans' sums meet in a merge kernel in span order: results do not depend on where pages lie or on other sequences' keys.
+// F32 queries and their probabilities are binary16 hi + lo pairs (two products each), K is converted as V is (the sums above begin
+// far from where they end: 1.8e-6 off instead of 6e-7), and a page's sums are added in the registers, as an addition of the matrix
+// instruction cuts at the sum's last bit.  Softmax in base 2; a column's reference moves only when a score passes it by 2^8, and P is
+// held 2^7 times, so that small probabilities stay normal numbers.
+// Results do not depend on where pages lie; how the work is cut, and with it the last bits, depends on the call's lengths.
 #include <math.h>
 
 #include <algorithm>
@@ -39,6 +43,10 @@ __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t o
     uint32_t r;
     asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(mask), "r"(other));
     return r;
+}
+// 64 + the nibbles of bits 4 .. 7 of both halves, times the scale, minus 72 times it
+__device__ __forceinline__ uint32_t value(uint32_t x, __half2 scale, __half2 minus72) {
+    return bits_of(__hfma2(half2_of(and_or(x, 0x00F000F0u, 0x54005400u)), scale, minus72));
 }
 // d = a b + c
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
@@ -75,28 +83,51 @@ __device__ __forceinline__ void store_value(const KvQ4Attention& a, long long at
     else asm volatile("{\n\t.reg .b16 t;\n\tcvt.rn.bf16.f32 t, %1;\n\tst.global.b16 [%0], t;\n\t}" ::"l"(static_cast<unsigned short*>(a.out) + at), "f"(x) : "memory");
 }
 
-// The rows of a sequence and the pages that a block of its columns sees.  Positions: row i is at base + i.
-struct Block {
-    int row0, n, base, cols, first_row, last_row;
-    int low, high;         // keys that some row of the block sees: low <= key < high
-    int page0, pages, per, spans;
+constexpr int kSetUp = 40;
+
+// A sequence in the list of work.  Its row i is at position base + i.
+struct Sequence {
+    int row0, n, base;
+    int page0, pages;      // that some row sees
+    int blocks;            // of columns
+    // Of an item, in pages: its set-up and fold, a chain of memory's latencies, take as long as kSetUp of them.  (Counted as 8, CTAs with
+    // many short items were the last ones by far: 40 sequences of four rows behind windows of 4,096 keys, a tenth of them with four
+    // keys, 264 us; as 24, 213; as 40, 172.)  One without keys writes its zeros.
+    __device__ __forceinline__ int length() const { return pages > 0 ? pages + kSetUp : 1; }
+    __device__ __forceinline__ long long weight(int kv_heads) const { return (long long)kv_heads * blocks * length(); }
 };
-__device__ __forceinline__ Block block_of(const KvQ4Attention& a, int s, int cb) {
+__device__ __forceinline__ Sequence sequence_of(const KvQ4Attention& a, int s) {
+    Sequence q;
+    const int group = a.q_heads / a.kv_heads;
+    q.row0 = max(a.cu_rows[s], 0);
+    q.n = max(0, min(a.cu_rows[s + 1], a.rows) - q.row0);
+    q.base = min(max(a.lengths[s], 0), a.pages_per_sequence * kQ4Page) - q.n;
+    const int high = max(0, q.base + q.n), low = a.window > 0 ? max(0, q.base - a.window + 1) : 0;
+    q.page0 = low / kQ4Page;
+    q.pages = high > low ? (high + kQ4Page - 1) / kQ4Page - q.page0 : 0;
+    const long long cols = (long long)min(q.n, a.max_rows) * group;
+    q.blocks = cols > a.tile_above ? 0 : (int)((cols + a.span_cols - 1) / a.span_cols);   // 0: the tile kernel's
+    return q;
+}
+// Pages per CTA of a list of `total`: whole rounds of the four warps
+__device__ __forceinline__ long long share_of(const KvQ4Attention& a, long long total) {
+    const long long even = (total + a.grid - 1) / a.grid;
+    return (max(even, (long long)a.least_pages) + kWarps - 1) / kWarps * kWarps;
+}
+// One item's columns
+struct Block {
+    int cols, flat0, first_row, last_row;
+    int low, high;         // keys that some row of the block sees: low <= key < high
+};
+__device__ __forceinline__ Block block_of(const KvQ4Attention& a, const Sequence& q, int cb) {
     Block b;
     const int group = a.q_heads / a.kv_heads;
-    b.row0 = max(a.cu_rows[s], 0);
-    b.n = min(a.cu_rows[s + 1], a.rows) - b.row0;
-    const int length = min(max(a.lengths[s], 0), a.pages_per_sequence * kQ4Page);
-    b.base = length - b.n;
-    b.cols = (long long)b.n * group > a.tile_above ? 0 : max(0, min(a.span_cols, b.n * group - cb * a.span_cols));   // 0: the tile kernel's
-    b.first_row = cb * a.span_cols / group;
-    b.last_row = (cb * a.span_cols + b.cols - 1) / group;
-    b.high = max(0, b.base + b.last_row + 1);
-    b.low = a.window > 0 ? max(0, b.base + b.first_row - a.window + 1) : 0;
-    b.page0 = b.low / kQ4Page;
-    b.pages = b.high > b.low ? (b.high + kQ4Page - 1) / kQ4Page - b.page0 : 0;
-    b.per = max(a.span_pages, (b.pages + a.max_spans - 1) / a.max_spans);
-    b.spans = max(1, (b.pages + b.per - 1) / b.per);
+    b.flat0 = cb * a.span_cols;
+    b.cols = min(a.span_cols, min(q.n, a.max_rows) * group - b.flat0);
+    b.first_row = b.flat0 / group;
+    b.last_row = (b.flat0 + b.cols - 1) / group;
+    b.high = max(0, q.base + b.last_row + 1);
+    b.low = a.window > 0 ? max(0, q.base + b.first_row - a.window + 1) : 0;
     return b;
 }
 
@@ -111,22 +142,93 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 && NT == 1 ? (PAIR ? 3 
     extern __shared__ __align__(128) unsigned char smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int group = a.q_heads / a.kv_heads;
-    // (span, sequence, kv head, column block), the last one fastest
-    int id = blockIdx.x;
-    const int cb = id % a.col_blocks; id /= a.col_blocks;
-    const int kvh = id % a.kv_heads; id /= a.kv_heads;
-    const int s = id % a.sequences, span = id / a.sequences;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const Block b = block_of(a, s, cb);
-    if (b.cols <= 0 || span >= b.spans) return;
-    const int begin = b.page0 + span * b.per, end = min(begin + b.per, b.page0 + b.pages);
+    // ---- where this CTA's run begins: the list's length before each sequence, a stretch of sequences per thread
+    __shared__ long long sums[kWarps];
+    __shared__ long long at_sequence_before;
+    __shared__ int at_sequence;
+    const int stretch = (a.sequences + kWarps * 32 - 1) / (kWarps * 32), s0 = min(a.sequences, (int)threadIdx.x * stretch), s1 = min(a.sequences, s0 + stretch);
+    long long mine_sum = 0;
+    for (int i = s0; i < s1; ++i) mine_sum += sequence_of(a, i).weight(a.kv_heads);
+    long long upto = mine_sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long other = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += other;
+    }
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    long long total = 0, before = upto - mine_sum;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += sums[w];
+        total += sums[w];
+    }
+    const long long share = share_of(a, total);
+    long long at = blockIdx.x * share;
+    const long long stop = min(total, at + share);
+    if (blockIdx.x == 0 && a.max_spans > 1) {   // for the merge
+        long long x = before;
+        for (int i = s0; i < s1; ++i) { a.prefix[i] = x; x += sequence_of(a, i).weight(a.kv_heads); }
+        if (threadIdx.x == 0) a.prefix[a.sequences] = total;
+    }
+    if (at >= stop) return;
+    if (before <= at && at < before + mine_sum) {
+        long long x = before;
+        int i = s0;
+        for (;; ++i) {
+            const long long w = sequence_of(a, i).weight(a.kv_heads);
+            if (at < x + w) break;
+            x += w;
+        }
+        at_sequence = i;
+        at_sequence_before = x;
+    }
+    __syncthreads();
+    int s = at_sequence;
+    long long s_before = at_sequence_before;
+    Sequence seq = sequence_of(a, s);
+    for (bool first_run = true; at < stop; first_run = false) {
+    while (at >= s_before + seq.weight(a.kv_heads)) {   // the next sequence that has work (`at` is inside of the list)
+        s_before += seq.weight(a.kv_heads);
+        seq = sequence_of(a, ++s);
+    }
+    const long long inside = at - s_before;
+    const int item = (int)(inside / seq.length()), offset = (int)(inside - (long long)item * seq.length());
+    const int kvh = item / seq.blocks, cb = item % seq.blocks, run = (int)min((long long)(seq.length() - offset), stop - at);
+    const bool whole = run == seq.length();
+    const Block b = block_of(a, seq, cb);
+    // the run's pages, those that the block sees
+    const int begin = max(seq.page0 + max(offset - kSetUp, 0), b.low / kQ4Page);
+    const int end = max(begin, min(seq.page0 + max(min(offset + run - kSetUp, seq.pages), 0), (b.high + kQ4Page - 1) / kQ4Page));
+    at += run;
+    if (begin == end) {   // none: zeros, or a share of the item that counts for nothing
+        for (int i = threadIdx.x; i < b.cols * REC; i += kWarps * 32) {
+            const int col = i / REC, d = i % REC, flat = b.flat0 + col;
+            if (!whole) a.partial[((2ll * blockIdx.x + (first_run ? 0 : 1)) * a.span_cols + col) * REC + d] = d == HD ? -INFINITY : 0.0f;
+            else if (d < HD) store_value(a, (seq.row0 + flat / group) * a.out_stride + (long long)(kvh * group + flat % group) * HD + d, 0.0f);
+        }
+        continue;
+    }
     const int mine = max(0, (end - begin - warp + kWarps - 1) / kWarps);   // this warp's pages
     const int32_t* table = a.page_tables + s * a.table_stride + begin + warp;
     const uint32_t ring = smem_at(smem) + warp * (RING * RECORD);
     const unsigned char* head = a.cache + (long long)kvh * RECORD;
     const long long page_stride = (long long)a.kv_heads * RECORD;
 
+    // the columns' queries, asked for before what the pages' addresses wait for
+    uint32_t raw[NT][NG][PAIR ? 8 : 4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int col = nt * 8 + g, flat = b.flat0 + col;
+#pragma unroll
+        for (int G = 0; G < NG; ++G) {
+#pragma unroll
+            for (int i = 0; i < (PAIR ? 8 : 4); ++i) raw[nt][G][i] = 0u;
+            if (col < b.cols) q4_load_raw(a.q, (seq.row0 + flat / group) * a.q_stride + (long long)(kvh * group + flat % group) * HD + 32 * G + 8 * t, a.vector_q, raw[nt][G]);
+        }
+    }
     // Page i of this warp: its number lies in lane i % 32; one outside of the arena is neither copied nor seen.
     int ids = lane < mine ? table[lane * kWarps] : -1;
     uint32_t good = 0;   // by i % 32
@@ -152,20 +254,16 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 && NT == 1 ? (PAIR ? 3 
 #pragma unroll
     for (int i = 0; i < RING - 1; ++i) issue(i);
 
-    // B fragments of Q^T: column 8 nt + g; of group G the dimensions 32 G + 8 t + {0, 4, 2, 6} and, 2^-4 times, {1, 5, 3, 7}
-    uint32_t qh[NT][NG][4], ql[PAIR ? NT : 1][PAIR ? NG : 1][4];
-    float start[NT][NG][2], factor[NT][2];
+    // B fragments of Q^T: column 8 nt + g; of group G the dimensions 32 G + 8 t + {0, 4, 2, 6} and, 2^-4 times (not PAIR), {1, 5, 3, 7}
+    uint32_t qh[NT][NG][4], ql[NT][PAIR ? NG : 1][4];
+    float start[NT][PAIR ? 1 : NG][2], factor[NT][2];
     int last[NT][2], lowest[NT][2];   // keys that columns 8 nt + 2 t + {0, 1} see
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int col = nt * 8 + g, flat = cb * a.span_cols + col;
-        const bool have = col < b.cols;
         float x[NG][8], top = 0.0f;
 #pragma unroll
         for (int G = 0; G < NG; ++G) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[G][i] = 0.0f;
-            if (have) q4_load8(a.q, (b.row0 + flat / group) * a.q_stride + (long long)(kvh * group + flat % group) * HD + 32 * G + 8 * t, a.type, a.vector_q, x[G]);
+            q4_values(raw[nt][G], a.type, x[G]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[G][i]));
         }
@@ -174,7 +272,7 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 && NT == 1 ? (PAIR ? 3 
         // 2^e brings the largest to [2^13, 2^14)
         const int e = top > 0.0f && top < INFINITY ? max(-126, min(126, 140 - (int)(__float_as_uint(top) >> 23))) : 0;
         const float up = __int_as_float((e + 127) << 23), down = __int_as_float((127 - e) << 23);
-        const float f = down * (a.scale * kLog2e * 16777216.0f);
+        const float f = down * (a.scale * kLog2e * (PAIR ? 1.0f : 16777216.0f));   // (codes are held 2^-24 times)
         factor[nt][0] = __shfl_sync(0xffffffffu, f, 8 * t);
         factor[nt][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
 #pragma unroll
@@ -182,32 +280,34 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 && NT == 1 ? (PAIR ? 3 
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) { x[G][i] *= up; sum += x[G][i]; }
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            sum *= -8.0f / 16777216.0f;
-            start[nt][G][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
-            start[nt][G][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+            if constexpr (!PAIR) {
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                sum *= -8.0f / 16777216.0f;
+                start[nt][G][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
+                start[nt][G][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+            }
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int i = (u & 1) * 2 + (u >> 1);   // 0, 2, 1, 3: the word's pairs are (i, i + 4)
-                const float m = (u >> 1) ? 0.0625f : 1.0f;
+                const float m = !PAIR && (u >> 1) ? 0.0625f : 1.0f;
                 const __half2 h = __floats2half2_rn(x[G][i] * m, x[G][i + 4] * m);
                 qh[nt][G][u] = bits_of(h);
                 if (PAIR) {
                     const float2 back = __half22float2(h);
-                    ql[PAIR ? nt : 0][PAIR ? G : 0][u] = bits_of(__floats2half2_rn(x[G][i] * m - back.x, x[G][i + 4] * m - back.y));
+                    ql[nt][PAIR ? G : 0][u] = bits_of(__floats2half2_rn(x[G][i] * m - back.x, x[G][i + 4] * m - back.y));
                 }
             }
         }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            const int at = nt * 8 + 2 * t + c;
-            last[nt][c] = at < b.cols ? b.base + (cb * a.span_cols + at) / group : -1;
+            const int column = nt * 8 + 2 * t + c;
+            last[nt][c] = column < b.cols ? seq.base + (b.flat0 + column) / group : -1;
             lowest[nt][c] = a.window > 0 ? last[nt][c] - a.window + 1 : 0;
         }
     }
     // keys that every column sees
-    const int all_low = a.window > 0 ? b.base + b.last_row - a.window + 1 : 0, all_high = b.base + b.first_row;
+    const int all_low = a.window > 0 ? seq.base + b.last_row - a.window + 1 : 0, all_high = seq.base + b.first_row;
 
     float o[NT][2 * NG][4], m[NT][2], l[NT][2];
 #pragma unroll
@@ -247,30 +347,36 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 && NT == 1 ? (PAIR ? 3 
                 for (int w = 0; w < WORDS; ++w) {
                     const int G = sub * WORDS + w;
                     const uint32_t x0 = w0[w] >> 8, x1 = w1[w] >> 8;
-                    const uint32_t even[4] = {w0[w] & 0x000F000Fu, w1[w] & 0x000F000Fu, x0 & 0x000F000Fu, x1 & 0x000F000Fu};
-                    const uint32_t odd[4] = {w0[w] & 0x00F000F0u, w1[w] & 0x00F000F0u, x0 & 0x00F000F0u, x1 & 0x00F000F0u};
-                    const float2 k0 = __half22float2(half2_of(s0[G >> 1])), k1 = __half22float2(half2_of(s1[G >> 1]));
-                    const float f0 = (G & 1) ? k0.y : k0.x, f1 = (G & 1) ? k1.y : k1.x;
+                    if constexpr (PAIR) {
+                        const __half2 minus72 = __float2half2_rn(-72.0f);
+                        const __half2 k0 = half2_of(__byte_perm(s0[G >> 1], 0u, (G & 1) ? 0x3232u : 0x1010u)), k1 = half2_of(__byte_perm(s1[G >> 1], 0u, (G & 1) ? 0x3232u : 0x1010u));
+                        const __half2 z0 = __hmul2(k0, minus72), z1 = __hmul2(k1, minus72);
+                        const uint32_t even[4] = {value(w0[w] * 16u, k0, z0), value(w1[w] * 16u, k1, z1), value(x0 * 16u, k0, z0), value(x1 * 16u, k1, z1)};
+                        const uint32_t odd[4] = {value(w0[w], k0, z0), value(w1[w], k1, z1), value(x0, k0, z0), value(x1, k1, z1)};
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        const float from[4] = {start[nt][G][0], start[nt][G][1], start[nt][G][0], start[nt][G][1]};
-                        float acc[4];
-                        if (PAIR) {
-                            const uint32_t(&lo)[4] = ql[PAIR ? nt : 0][PAIR ? G : 0];
-                            const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                            mma(acc, even, lo[0], lo[1], zero);
-                            mma(acc, odd, lo[2], lo[3], acc);
-                            float high[4];
-                            mma(high, even, qh[nt][G][0], qh[nt][G][1], from);
-                            mma(high, odd, qh[nt][G][2], qh[nt][G][3], high);
+                        for (int nt = 0; nt < NT; ++nt) {
+                            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            mma(acc, even, ql[nt][G][0], ql[nt][G][1], acc);
+                            mma(acc, odd, ql[nt][G][2], ql[nt][G][3], acc);
+                            mma(acc, even, qh[nt][G][0], qh[nt][G][1], acc);
+                            mma(acc, odd, qh[nt][G][2], qh[nt][G][3], acc);
 #pragma unroll
-                            for (int u = 0; u < 4; ++u) acc[u] += high[u];
-                        } else {
+                            for (int u = 0; u < 4; ++u) sc[nt][u] += acc[u];
+                        }
+                    } else {
+                        const uint32_t even[4] = {w0[w] & 0x000F000Fu, w1[w] & 0x000F000Fu, x0 & 0x000F000Fu, x1 & 0x000F000Fu};
+                        const uint32_t odd[4] = {w0[w] & 0x00F000F0u, w1[w] & 0x00F000F0u, x0 & 0x00F000F0u, x1 & 0x00F000F0u};
+                        const float2 k0 = __half22float2(half2_of(s0[G >> 1])), k1 = __half22float2(half2_of(s1[G >> 1]));
+                        const float f0 = (G & 1) ? k0.y : k0.x, f1 = (G & 1) ? k1.y : k1.x;
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const float from[4] = {start[nt][G][0], start[nt][G][1], start[nt][G][0], start[nt][G][1]};
+                            float acc[4];
                             mma(acc, even, qh[nt][G][0], qh[nt][G][1], from);
                             mma(acc, odd, qh[nt][G][2], qh[nt][G][3], acc);
+                            sc[nt][0] = fmaf(acc[0], f0, sc[nt][0]); sc[nt][1] = fmaf(acc[1], f0, sc[nt][1]);
+                            sc[nt][2] = fmaf(acc[2], f1, sc[nt][2]); sc[nt][3] = fmaf(acc[3], f1, sc[nt][3]);
                         }
-                        sc[nt][0] = fmaf(acc[0], f0, sc[nt][0]); sc[nt][1] = fmaf(acc[1], f0, sc[nt][1]);
-                        sc[nt][2] = fmaf(acc[2], f1, sc[nt][2]); sc[nt][3] = fmaf(acc[3], f1, sc[nt][3]);
                     }
                 }
             }
@@ -345,9 +451,9 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 && NT == 1 ? (PAIR ? 3 
                 for (int w = 0; w < WORDS; ++w) {
                     const int G = sub * WORDS + w;
                     const __half2 a0 = half2_of(s0[G]), a1 = half2_of(s1[G]), b0 = __hmul2(a0, minus72), b1 = __hmul2(a1, minus72);
-                    auto value = [&](uint32_t x, __half2 sa, __half2 sb) { return bits_of(__hfma2(half2_of(and_or(x, 0x00F000F0u, 0x54005400u)), sa, sb)); };
-                    const uint32_t lower[4] = {value(w0[w] << 4, a0, b0), value(w0[w], a0, b0), value(w1[w] << 4, a1, b1), value(w1[w], a1, b1)};
-                    const uint32_t upper[4] = {value(w0[w] >> 4, a0, b0), value(w0[w] >> 8, a0, b0), value(w1[w] >> 4, a1, b1), value(w1[w] >> 8, a1, b1)};
+                    const uint32_t u0 = w0[w] >> 8, u1 = w1[w] >> 8;   // (to the left by a multiplication, which runs beside the logic)
+                    const uint32_t lower[4] = {value(w0[w] * 16u, a0, b0), value(w0[w], a0, b0), value(w1[w] * 16u, a1, b1), value(w1[w], a1, b1)};
+                    const uint32_t upper[4] = {value(u0 * 16u, a0, b0), value(u0, a0, b0), value(u1 * 16u, a1, b1), value(u1, a1, b1)};
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         if (PAIR) {   // a page's sum by itself: the instruction cuts at the last bit of what it adds to
@@ -396,74 +502,79 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 && NT == 1 ? (PAIR ? 3 
         }
     }
     __syncthreads();
-    const int live = min(kWarps, end - begin);
+    const int live = min(kWarps, end - begin);   // warps that have pages
     const float* recs = reinterpret_cast<const float*>(smem);
     for (int col = warp; col < b.cols; col += kWarps) {
-        const int flat = cb * a.span_cols + col, row = b.row0 + flat / group, qh_index = kvh * group + flat % group;
+        const int flat = b.flat0 + col, row = seq.row0 + flat / group, qh_index = kvh * group + flat % group;
         float top = -INFINITY;
         for (int w = 0; w < live; ++w) top = fmaxf(top, recs[w * kWarpFloats + col * REC + HD]);
-        float acc[HD / 32], total = 0.0f;
+        float acc[HD / 32], sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < HD / 32; ++i) acc[i] = 0.0f;
         for (int w = 0; w < live; ++w) {
             const float mw = recs[w * kWarpFloats + col * REC + HD], fw = mw == -INFINITY ? 0.0f : exp2_approx(mw - top);
-            total = fmaf(recs[w * kWarpFloats + col * REC + HD + 1], fw, total);
+            sum = fmaf(recs[w * kWarpFloats + col * REC + HD + 1], fw, sum);
 #pragma unroll
             for (int i = 0; i < HD / 32; ++i) acc[i] = fmaf(recs[w * kWarpFloats + col * REC + lane + 32 * i], fw, acc[i]);
         }
-        if (b.spans == 1) {
-            const long long at = row * a.out_stride + (long long)qh_index * HD;
+        if (whole) {
+            const long long to = row * a.out_stride + (long long)qh_index * HD;
 #pragma unroll
-            for (int i = 0; i < HD / 32; ++i) store_value(a, at + lane + 32 * i, total > 0.0f || total != total ? acc[i] / total : 0.0f);
-        } else {
-            float* pp = a.partial + (((long long)row * a.q_heads + qh_index) * a.max_spans + span) * REC;
+            for (int i = 0; i < HD / 32; ++i) store_value(a, to + lane + 32 * i, sum > 0.0f || sum != sum ? acc[i] / sum : 0.0f);
+        } else {   // the CTA's first run in its first place, its last in the second: those between are whole items
+            float* pp = a.partial + ((2ll * blockIdx.x + (first_run ? 0 : 1)) * a.span_cols + col) * REC;
 #pragma unroll
             for (int i = 0; i < HD / 32; ++i) pp[lane + 32 * i] = acc[i];
-            if (lane == 0) { pp[HD] = top; pp[HD + 1] = total; }
+            if (lane == 0) { pp[HD] = top; pp[HD + 1] = sum; }
         }
+    }
+    __syncthreads();   // the rings are free again
     }
 }
 
-// out = sum_s acc_s 2^(m_s - M) / sum_s l_s 2^(m_s - M): four warps per (row, query head), warp w spans w, w + 4, .., then the warps in order.
+// out = sum_r acc_r 2^(m_r - M) / sum_r l_r 2^(m_r - M) over an item's runs: four warps per (item, column), warp w runs w, w + 4, ..,
+// then the warps in order.
 template <int HD>
 __global__ void __launch_bounds__(kWarps * 32) kvq4_merge_kernel(const KvQ4Attention a) {
     constexpr int DPL = HD / 32, REC = HD + 2, GROUP = 4;
     __shared__ float sums[kWarps][HD + 1];
-    const int row = (int)blockIdx.x / a.q_heads, qh = (int)blockIdx.x % a.q_heads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int group = a.q_heads / a.kv_heads;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = a.q_heads / a.kv_heads;
+    int id = blockIdx.x;
+    const int col = id % a.merge_cols; id /= a.merge_cols;
+    const int cb = id % a.col_blocks; id /= a.col_blocks;
+    const int kvh = id % a.kv_heads, s = id / a.kv_heads;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    int s = 0, above = a.sequences;   // the last sequence that begins at or before the row
-    while (above - s > 1) {
-        const int mid = (s + above) / 2;
-        if (a.cu_rows[mid] <= row) s = mid; else above = mid;
-    }
-    if (row < a.cu_rows[s] || row >= a.cu_rows[s + 1]) return;
-    const int flat = (row - a.cu_rows[s]) * group + qh % group;
-    if (flat / a.span_cols >= a.col_blocks) return;   // more rows than the call said
-    const Block b = block_of(a, s, flat / a.span_cols);
-    if (b.cols <= 0 || b.spans <= 1) return;   // written by the tile or the span kernel
-    const float* pp = a.partial + ((long long)row * a.q_heads + qh) * a.max_spans * REC;
+    const Sequence q = sequence_of(a, s);
+    if (cb >= q.blocks) return;
+    const Block b = block_of(a, q, cb);
+    if (col >= b.cols) return;
+    const long long share = share_of(a, __ldcg(a.prefix + a.sequences)), from = __ldcg(a.prefix + s) + (long long)(kvh * q.blocks + cb) * q.length();
+    const int c0 = (int)(from / share), runs = (int)((from + q.length() - 1) / share) - c0 + 1;
+    if (runs <= 1) return;   // written by the span kernel
+    // the item's run in CTA c0 is that one's last, in the others their first
+    const bool last_of_c0 = from > c0 * share;
+    auto record = [&](int r) { return a.partial + ((2ll * (c0 + r) + (r == 0 && last_of_c0 ? 1 : 0)) * a.span_cols + col) * REC; };
     float top = -INFINITY;
-    for (int i = lane; i < b.spans; i += 32) top = fmaxf(top, __ldcg(pp + (long long)i * REC + HD));
+    for (int r = lane; r < runs; r += 32) top = fmaxf(top, __ldcg(record(r) + HD));
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
     float sum[DPL], denom = 0.0f;
 #pragma unroll
     for (int i = 0; i < DPL; ++i) sum[i] = 0.0f;
-    for (int s0 = warp; s0 < b.spans; s0 += kWarps * GROUP) {
+    for (int r0 = warp; r0 < runs; r0 += kWarps * GROUP) {
         float v[GROUP][DPL], mx[GROUP], lx[GROUP];
 #pragma unroll
         for (int u = 0; u < GROUP; ++u) {
-            const int at = s0 + kWarps * u;
-            const float* rec = pp + (long long)at * REC;
+            const int r = r0 + kWarps * u;
+            const float* rec = record(min(r, runs - 1));
 #pragma unroll
-            for (int i = 0; i < DPL; ++i) v[u][i] = at < b.spans ? __ldcg(rec + lane + 32 * i) : 0.0f;
-            mx[u] = at < b.spans ? __ldcg(rec + HD) : -INFINITY;
-            lx[u] = at < b.spans ? __ldcg(rec + HD + 1) : 0.0f;
+            for (int i = 0; i < DPL; ++i) v[u][i] = __ldcg(rec + lane + 32 * i);
+            mx[u] = r < runs ? __ldcg(rec + HD) : -INFINITY;
+            lx[u] = __ldcg(rec + HD + 1);
         }
 #pragma unroll
         for (int u = 0; u < GROUP; ++u) {
-            const float w = mx[u] == -INFINITY ? 0.0f : exp2_approx(mx[u] - top);
+            const float w = mx[u] == -INFINITY ? 0.0f : exp2_approx(mx[u] - top);   // past the last run, without keys, or lost in NaN (which 0 x keeps)
             denom = fmaf(lx[u], w, denom);
 #pragma unroll
             for (int i = 0; i < DPL; ++i) sum[i] = fmaf(v[u][i], w, sum[i]);
@@ -473,16 +584,18 @@ __global__ void __launch_bounds__(kWarps * 32) kvq4_merge_kernel(const KvQ4Atten
     for (int i = 0; i < DPL; ++i) sums[warp][lane + 32 * i] = sum[i];
     if (lane == 0) sums[warp][HD] = denom;
     __syncthreads();
-    const float total = ((sums[0][HD] + sums[1][HD]) + sums[2][HD]) + sums[3][HD];
+    const float all = ((sums[0][HD] + sums[1][HD]) + sums[2][HD]) + sums[3][HD];
+    const int flat = b.flat0 + col;
+    const long long to = (q.row0 + flat / group) * a.out_stride + (long long)(kvh * group + flat % group) * HD;
     for (int d = threadIdx.x; d < HD; d += kWarps * 32) {
         const float value = ((sums[0][d] + sums[1][d]) + sums[2][d]) + sums[3][d];
-        store_value(a, row * a.out_stride + (long long)qh * HD + d, total > 0.0f || total != total ? value / total : 0.0f);
+        store_value(a, to + d, all > 0.0f || all != all ? value / all : 0.0f);
     }
 }
 
 bool aligned16(const void* p, long long stride, int size) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride * size % 16 == 0; }
 
-// How a launch is split: columns per CTA and spans.
+// Columns per CTA, and how many CTAs share the list.
 void plan_spans(KvQ4Attention& a) {
     const int group = a.q_heads / a.kv_heads;
     a.tile_above = a.head_dim == 256 ? 0x7fffffff : 32;
@@ -490,22 +603,14 @@ void plan_spans(KvQ4Attention& a) {
     // 16 columns share a page's conversion; with heads of 256 their sums do not fit in the registers (1,080 bytes of spills)
     a.span_cols = cols <= 8 || a.head_dim == 256 ? 8 : 16;
     a.col_blocks = (cols + a.span_cols - 1) / a.span_cols;
-    const int keys = a.window > 0 ? (int)std::min<long long>(a.max_keys, (long long)a.window + a.max_rows + kQ4Page) : a.max_keys;
-    const int pages = std::max(1, (keys + kQ4Page - 1) / kQ4Page);
-    const long long items = (long long)a.sequences * a.kv_heads * a.col_blocks;
+    a.merge_cols = std::min(cols, a.span_cols);
+    const long long keys = a.window > 0 ? std::min<long long>(a.max_keys, (long long)a.window + a.max_rows + kQ4Page) : a.max_keys;
+    const long long pages = std::max(1ll, (keys + kQ4Page - 1) / kQ4Page), items = (long long)a.sequences * a.kv_heads * a.col_blocks;
     const long long resident = (long long)kvq4_sm_count() * (a.head_dim <= 128 && a.span_cols == 8 ? (a.type == kQ4F32 ? 3 : 4) : 2);
-    // F32: a sum of at most 16 pages per warp, as each addition of the matrix instruction cuts at the sum's last bit
-    const int most = a.type == kQ4F32 ? 64 : 1 << 20;
-    // the fewest page-times of the busiest CTA, with a span's set-up and fold counted as eight pages of a warp
-    float best = 0.0f;
-    a.span_pages = std::min(pages, most);
-    for (int spans = (pages + most - 1) / most; spans <= std::min(512, (pages + 3) / 4); spans += std::max(1, spans / 8)) {
-        const int per = (pages + spans - 1) / spans;
-        const long long waves = (items * spans + resident - 1) / resident;
-        const float cost = (float)waves * ((float)((per + 3) / 4) + 8.0f) + (spans > 1 ? 6.0f + 0.5f * (float)(spans / 16) : 0.0f);
-        if (best == 0.0f || cost < best) { best = cost; a.span_pages = per; }
-    }
-    a.max_spans = (pages + a.span_pages - 1) / a.span_pages;
+    a.least_pages = 3 * kWarps;
+    a.grid = (int)std::max(1ll, std::min(resident, (items * pages + a.least_pages - 1) / a.least_pages));
+    a.max_spans = 2;   // an item may be cut, unless one CTA has all
+    if (a.grid == 1) a.max_spans = 1;
 }
 
 template <typename Kernel>
@@ -537,7 +642,7 @@ cudaError_t launch_spans(cudaStream_t stream, const KvQ4Attention& a) {
         if (e != cudaSuccess) return e;
         configured[dev] = true;
     }
-    return launch(stream, kvq4_span_kernel<HD, NT, PAIR>, (long long)a.max_spans * a.sequences * a.kv_heads * a.col_blocks, smem, a, false);
+    return launch(stream, kvq4_span_kernel<HD, NT, PAIR>, a.grid, smem, a, false);
 }
 
 template <int HD>
@@ -546,7 +651,7 @@ cudaError_t launch_hd(cudaStream_t stream, const KvQ4Attention& a) {
     const bool pair = a.type == kQ4F32;
     cudaError_t e = a.span_cols == 8 ? (pair ? launch_spans<HD, 1, true>(stream, a) : launch_spans<HD, 1, false>(stream, a))
                                      : (pair ? launch_spans<HD, WIDE, true>(stream, a) : launch_spans<HD, WIDE, false>(stream, a));
-    if (e == cudaSuccess && a.max_spans > 1) e = launch(stream, kvq4_merge_kernel<HD>, (long long)a.rows * a.q_heads, 0, a, true);
+    if (e == cudaSuccess && a.max_spans > 1) e = launch(stream, kvq4_merge_kernel<HD>, (long long)a.sequences * a.kv_heads * a.col_blocks * a.merge_cols, 0, a, true);
     return e;
 }
 
@@ -565,8 +670,9 @@ namespace {
 // Bytes of the spans' sums, and behind them room for the tile kernel's operands: at most kScratchMost, or what the sequences with
 // enough rows can need.
 constexpr size_t kScratchMost = 512u << 20;
+size_t prefix_bytes(const KvQ4Attention& a) { return ((size_t)a.sequences + 1) * sizeof(long long); }
 size_t partial_bytes(const KvQ4Attention& a) {
-    const size_t n = a.max_spans > 1 ? (size_t)a.rows * a.q_heads * a.max_spans * (a.head_dim + 2) * sizeof(float) : 0;
+    const size_t n = a.max_spans > 1 ? prefix_bytes(a) + (size_t)a.grid * 2 * a.span_cols * (a.head_dim + 2) * sizeof(float) : 0;
     return (n + 255) / 256 * 256;
 }
 int wanted_tiles(const KvQ4Attention& a) {
@@ -590,7 +696,10 @@ cudaError_t launch_kvq4_attention(cudaStream_t stream, KvQ4Attention a) {
     plan_spans(a);
     const size_t sums = partial_bytes(a);
     if (a.partial_bytes < sums) return cudaErrorInvalidValue;
-    a.scratch = reinterpret_cast<unsigned char*>(a.partial) + sums;
+    unsigned char* scratch = reinterpret_cast<unsigned char*>(a.partial);
+    a.prefix = reinterpret_cast<long long*>(scratch);
+    a.partial = reinterpret_cast<float*>(scratch + prefix_bytes(a));
+    a.scratch = scratch + sums;
     a.scratch_tiles = (int)std::min<size_t>((size_t)wanted_tiles(a), (a.partial_bytes - sums) / ((size_t)512 * a.head_dim * a.kv_heads));
     const int size = a.type == kQ4F32 ? 4 : 2;
     a.vector_q = aligned16(a.q, a.q_stride, size);

@@ -524,7 +524,7 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
                 for (int p = 0; p < PP; ++p) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) x[p][i] = 0.0f;
-                    if (r < live_rows) q4_load8(a.q, (w.row0 + (flat0 + r) / group) * a.q_stride + (long long)(kvh * group + (flat0 + r) % group) * HD + (p * 4 + pc) * 8, a.type, a.vector_q, x[p]);
+                    if (r < live_rows) q4_load8<PAIR>(a.q, (w.row0 + (flat0 + r) / group) * a.q_stride + (long long)(kvh * group + (flat0 + r) % group) * HD + (p * 4 + pc) * 8, a.type, a.vector_q, x[p]);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[p][i]));
                 }

@@ -84,11 +84,15 @@ def test_nothing_to_do_is_not_an_error(lib):
     assert lib.ribn_b200_kvq4_attention(0, None, _args(sequences=0, lengths=None)) == 0
 
 
-def test_workspace_covers_long_and_wide_calls(lib):
-    """A split launch asks for (head_dim + 2) floats per row, head and span; what a call cannot use is not asked for."""
-    one = lib.ribn_b200_kvq4_workspace(_args(sequences=1, rows=1, max_keys=65536, pages_per_sequence=4096))
-    assert one > 0 and one % (16 * 130 * 4) == 0
-    assert lib.ribn_b200_kvq4_workspace(_args(sequences=1, rows=1, max_keys=16)) == 0
+def test_workspace_follows_the_call(lib):
+    """Scratch for what CTAs share of an item, and for the operands of sequences with many rows; none where one CTA does all."""
+    ask = lambda **change: lib.ribn_b200_kvq4_workspace(_args(**change))  # noqa: E731
+    assert ask(sequences=1, rows=1, q_heads=1, kv_heads=1, max_keys=16) == 0
+    small, long = ask(sequences=1, rows=1, max_keys=1024), ask(sequences=1, rows=1, max_keys=65536, pages_per_sequence=4096)
+    assert 0 < small < long < 32 << 20
+    # one sequence of 500 rows behind 1,000 keys: K and V of ten blocks of 128 keys as binary16, and no more than half a GB for any call
+    assert ask(sequences=1, rows=500, max_rows=500, max_keys=1000) >= 8 * 8 * 128 * 128 * 4
+    assert ask(sequences=64, rows=60000, max_rows=2000, max_keys=1 << 20) < 640 << 20
 
 
 @pytest.mark.parametrize("head_dim", [64, 128, 256])
