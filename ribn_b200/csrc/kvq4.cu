@@ -13,6 +13,8 @@ namespace ribn {
 
 namespace {
 
+constexpr unsigned kRowThreads = 256;
+
 __device__ __forceinline__ uint32_t bits_of(__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); }
 
 // Eight values that binary16 holds exactly
@@ -39,19 +41,37 @@ __device__ __forceinline__ void store8(void* base, long long at, const __half2 (
     }
 }
 
-// Where a row's eight dimensions lie: piece p of head_dim / 8.
+// Where a thread's eight dimensions lie: piece p of head_dim / 8 of `many` rows, `row` the first and `step` from one to the next.  A block
+// has `many` times some rows, or 256 pieces of as many.  Calls with many rows give a thread four, whose loads travel together.
 struct Piece {
-    long long row;
+    long long row, step;
     int head, which, p;   // which: 0 K, 1 V
+    bool inside;
 };
-__device__ __forceinline__ Piece piece_of(long long id, int kv_heads, int pieces) {
+__device__ __forceinline__ Piece piece_of(const KvQ4Rows& a, int many) {
+    // (32-bit arithmetic throughout: with three 64-bit divisions a thread 16,384 rows took 37 us to read back)
+    const int log_pieces = a.head_dim == 64 ? 3 : a.head_dim == 128 ? 4 : 5;
+    const unsigned per_row = (unsigned)(2 * a.kv_heads) << log_pieces;
     Piece r;
-    r.p = (int)(id % pieces);
-    const long long rest = id / pieces;
-    r.head = (int)(rest % kv_heads);
-    const long long more = rest / kv_heads;
-    r.which = (int)(more & 1);
-    r.row = more >> 1;
+    unsigned rest;
+    if (per_row <= kRowThreads) {
+        const unsigned rows = kRowThreads / per_row, mine = threadIdx.x / per_row;
+        r.row = (long long)blockIdx.x * rows * many + mine;
+        r.step = rows;
+        rest = threadIdx.x - mine * per_row;
+        r.inside = mine < rows;
+    } else {
+        const unsigned blocks = (per_row + kRowThreads - 1) / kRowThreads, row = blockIdx.x / blocks;
+        r.row = (long long)row * many;
+        r.step = 1;
+        rest = (blockIdx.x - row * blocks) * kRowThreads + threadIdx.x;
+        r.inside = rest < per_row;
+    }
+    if (!r.inside) rest = 0;
+    r.p = (int)(rest & ((1u << log_pieces) - 1));
+    const unsigned more = rest >> log_pieces;
+    r.which = more >= (unsigned)a.kv_heads;
+    r.head = (int)(r.which ? more - (unsigned)a.kv_heads : more);
     return r;
 }
 
@@ -92,19 +112,8 @@ __device__ __forceinline__ uint32_t scatter_nibbles(uint32_t halves, int i, int 
     return r;
 }
 
-template <int TYPE>
-__global__ void __launch_bounds__(256) kvq4_append_kernel(const KvQ4Rows a, const bool vector) {
-    const int pieces = a.head_dim / 8, lane = threadIdx.x & 31;
-    const long long total = a.rows * a.kv_heads * 2 * pieces;   // a multiple of eight: groups of four lanes stay whole
-    const long long id = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    const bool inside = id < total;
-    const Piece at = piece_of(inside ? id : 0, a.kv_heads, pieces);
-    const long long slot = a.slots[at.row];
-    const bool live = inside && slot >= 0 && slot < a.pages * kQ4Page;
-    float x[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-    if (live) q4_load8<TYPE == kQ4F32>(at.which ? a.v : a.k, at.row * (at.which ? a.v_stride : a.k_stride) + (long long)at.head * a.head_dim + at.p * 8, TYPE, vector, x);
+// The word of codes (nibble i: value i) of a thread's eight values and the scale of its group's 32, which four neighbouring threads have
+__device__ __forceinline__ uint32_t quantise8(float (&x)[8], int lane, uint32_t& scale_bits) {
     float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -118,7 +127,8 @@ __global__ void __launch_bounds__(256) kvq4_append_kernel(const KvQ4Rows a, cons
         top = fabsf(high) > fabsf(low) ? high : low;
     }
     const uint32_t raw = __half_as_ushort(__float2half_rn(top * -0.125f));
-    const uint32_t size = min(((raw & 0x7fffu) + 8u) & ~15u, 0x6300u), scale_bits = size | (raw & 0x8000u);
+    const uint32_t size = min(((raw & 0x7fffu) + 8u) & ~15u, 0x6300u);
+    scale_bits = size | (raw & 0x8000u);
     const float d = __half2float(__ushort_as_half((unsigned short)size)), inv = d > 0.0f ? 1.0f / d : 0.0f, half = 0.5f * d;
     uint32_t word = 0;
 #pragma unroll
@@ -129,79 +139,140 @@ __global__ void __launch_bounds__(256) kvq4_append_kernel(const KvQ4Rows a, cons
         q += d > 0.0f ? (rest >= half ? 1.0f : rest < -half ? -1.0f : 0.0f) : 0.0f;
         word |= (uint32_t)((int)fminf(fmaxf(q, -8.0f), 7.0f) + 8) << (4 * i);
     }
-    const int i4 = at.p & 3, G = at.p >> 2;
-    const uint32_t halves = gather_nibbles(word, i4, lane);
-    if (!live) return;
-    const int j = (int)(slot & (kQ4Page - 1));
-    unsigned char* record = a.cache + ((slot >> 4) * a.kv_heads + at.head) * q4_record(a.head_dim);
-    if (at.which == 0) {
-        *reinterpret_cast<uint32_t*>(record + k_word_at(a.head_dim, j, at.p)) = word;
-        if (i4 == 0) *reinterpret_cast<unsigned short*>(record + k_scale_at(a.head_dim, j, G)) = (unsigned short)scale_bits;
-    } else {
-        *reinterpret_cast<unsigned short*>(record + v_word_at(a.head_dim, j, G, 2 * i4)) = (unsigned short)halves;
-        *reinterpret_cast<unsigned short*>(record + v_word_at(a.head_dim, j, G, 2 * i4 + 1)) = (unsigned short)(halves >> 16);
-        if (i4 == 0) *reinterpret_cast<unsigned short*>(record + v_scale_at(a.head_dim, j, G)) = (unsigned short)scale_bits;
+    return word;
+}
+
+template <int TYPE, int MANY>
+__global__ void __launch_bounds__(kRowThreads) kvq4_append_kernel(const KvQ4Rows a, const bool vector) {
+    const int lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const Piece at = piece_of(a, MANY);   // a row has a multiple of eight: groups of four lanes are of one group of dimensions
+    constexpr int WORDS = TYPE == kQ4F32 ? 8 : 4;
+    uint32_t raw[MANY][WORDS];
+    int slot[MANY];
+#pragma unroll
+    for (int u = 0; u < MANY; ++u) {
+        const long long row = at.row + u * at.step;
+        const bool inside = at.inside && row < a.rows;
+        slot[u] = inside ? a.slots[row] : -1;
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) raw[u][i] = 0u;
+        if (inside) q4_load_raw(at.which ? a.v : a.k, row * (at.which ? a.v_stride : a.k_stride) + (long long)at.head * a.head_dim + at.p * 8, vector, raw[u]);
+    }
+    const int i4 = lane & 3, G = at.p >> 2;
+#pragma unroll
+    for (int u = 0; u < MANY; ++u) {
+        float x[8];
+        q4_values(raw[u], TYPE, x);
+        uint32_t scale_bits;
+        const uint32_t word = quantise8(x, lane, scale_bits), halves = gather_nibbles(word, i4, lane);
+        if (slot[u] < 0 || slot[u] >= a.pages * kQ4Page) continue;   // (the shuffles above are done)
+        const int j = slot[u] & (kQ4Page - 1);
+        unsigned char* record = a.cache + ((long long)(slot[u] >> 4) * a.kv_heads + at.head) * q4_record(a.head_dim);
+        if (at.which == 0) {
+            *reinterpret_cast<uint32_t*>(record + k_word_at(a.head_dim, j, at.p)) = word;
+            if (i4 == 0) *reinterpret_cast<unsigned short*>(record + k_scale_at(a.head_dim, j, G)) = (unsigned short)scale_bits;
+        } else {
+            *reinterpret_cast<unsigned short*>(record + v_word_at(a.head_dim, j, G, 2 * i4)) = (unsigned short)halves;
+            *reinterpret_cast<unsigned short*>(record + v_word_at(a.head_dim, j, G, 2 * i4 + 1)) = (unsigned short)(halves >> 16);
+            if (i4 == 0) *reinterpret_cast<unsigned short*>(record + v_scale_at(a.head_dim, j, G)) = (unsigned short)scale_bits;
+        }
     }
 }
 
-template <int TYPE>
-__global__ void __launch_bounds__(256) kvq4_read_kernel(const KvQ4Rows a) {
-    const int pieces = a.head_dim / 8, lane = threadIdx.x & 31;
-    const long long total = a.rows * a.kv_heads * 2 * pieces;
-    const long long id = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    const bool inside = id < total;
-    const Piece at = piece_of(inside ? id : 0, a.kv_heads, pieces);
-    const long long slot = a.slots[at.row];
-    const bool live = inside && slot >= 0 && slot < a.pages * kQ4Page;
-    const int i4 = at.p & 3, G = at.p >> 2, j = (int)(slot & (kQ4Page - 1));
-    const unsigned char* record = a.cache + (live ? ((slot >> 4) * a.kv_heads + at.head) * q4_record(a.head_dim) : 0);
-    uint32_t word = 0x88888888u, scale = 0;
-    if (live) {
-        if (at.which == 0) {
-            word = *reinterpret_cast<const uint32_t*>(record + k_word_at(a.head_dim, j, at.p));
-            scale = *reinterpret_cast<const unsigned short*>(record + k_scale_at(a.head_dim, j, G));
-        } else {
-            word = (uint32_t)*reinterpret_cast<const unsigned short*>(record + v_word_at(a.head_dim, j, G, 2 * i4)) |
-                   (uint32_t)*reinterpret_cast<const unsigned short*>(record + v_word_at(a.head_dim, j, G, 2 * i4 + 1)) << 16;
-            scale = *reinterpret_cast<const unsigned short*>(record + v_scale_at(a.head_dim, j, G));
+template <int TYPE, int MANY>
+__global__ void __launch_bounds__(kRowThreads) kvq4_read_kernel(const KvQ4Rows a) {
+    const int lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const Piece at = piece_of(a, MANY);
+    const int i4 = lane & 3, G = at.p >> 2;
+    int slot[MANY];
+    uint32_t word[MANY], scale[MANY];
+#pragma unroll
+    for (int u = 0; u < MANY; ++u) {
+        const long long row = at.row + u * at.step;
+        slot[u] = at.inside && row < a.rows ? a.slots[row] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < MANY; ++u) {
+        const int j = slot[u] & (kQ4Page - 1);
+        word[u] = 0x88888888u;
+        scale[u] = 0;
+        if (slot[u] >= 0 && slot[u] < a.pages * kQ4Page) {
+            const unsigned char* record = a.cache + ((long long)(slot[u] >> 4) * a.kv_heads + at.head) * q4_record(a.head_dim);
+            if (at.which == 0) {
+                word[u] = *reinterpret_cast<const uint32_t*>(record + k_word_at(a.head_dim, j, at.p));
+                scale[u] = *reinterpret_cast<const unsigned short*>(record + k_scale_at(a.head_dim, j, G));
+            } else {
+                word[u] = (uint32_t)*reinterpret_cast<const unsigned short*>(record + v_word_at(a.head_dim, j, G, 2 * i4)) |
+                          (uint32_t)*reinterpret_cast<const unsigned short*>(record + v_word_at(a.head_dim, j, G, 2 * i4 + 1)) << 16;
+                scale[u] = *reinterpret_cast<const unsigned short*>(record + v_scale_at(a.head_dim, j, G));
+            }
         }
     }
-    const uint32_t back = scatter_nibbles(word, i4, lane);
-    if (at.which != 0) word = back;
-    const __half2 s = __half2half2(__ushort_as_half((unsigned short)scale)), shift = __float2half2_rn(1032.0f);
-    __half2 x[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {   // 1024 + code, exact
-        const uint32_t pair = 0x64006400u | ((word >> (8 * i)) & 15u) | ((word >> (8 * i + 4)) & 15u) << 16;
-        x[i] = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&pair), shift), s);
+    for (int u = 0; u < MANY; ++u) {
+        const uint32_t back = scatter_nibbles(word[u], i4, lane), w = at.which ? back : word[u];
+        const __half2 s = __half2half2(__ushort_as_half((unsigned short)scale[u])), shift = __float2half2_rn(1032.0f);
+        __half2 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {   // 1024 + code, exact
+            const uint32_t pair = 0x64006400u | ((w >> (8 * i)) & 15u) | ((w >> (8 * i + 4)) & 15u) << 16;
+            x[i] = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&pair), shift), s);
+        }
+        const long long row = at.row + u * at.step;
+        if (at.inside && row < a.rows) {
+            store8<TYPE>(const_cast<void*>(at.which ? a.v : a.k), row * (at.which ? a.v_stride : a.k_stride) + (long long)at.head * a.head_dim + at.p * 8, x);
+        }
     }
-    if (inside) store8<TYPE>(const_cast<void*>(at.which ? a.v : a.k), at.row * (at.which ? a.v_stride : a.k_stride) + (long long)at.head * a.head_dim + at.p * 8, x);
 }
 
 bool aligned16(const void* p, long long stride, int size) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride * size % 16 == 0; }
+
+// Early launch: the kernel's blocks stand ready when the one before ends (each waits for it before it reads anything).
+template <typename Kernel, typename... Args>
+cudaError_t launch_rows(cudaStream_t stream, Kernel kernel, const KvQ4Rows& a, int many, Args... more) {
+    const long long per_row = 2ll * a.kv_heads * (a.head_dim / 8);
+    const long long together = (per_row <= kRowThreads ? kRowThreads / per_row : 1) * many;   // rows of a block
+    const long long blocks = (a.rows + together - 1) / together * (per_row <= kRowThreads ? 1 : (per_row + kRowThreads - 1) / kRowThreads);
+    if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(kRowThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, a, more...);
+}
+bool many_rows(const KvQ4Rows& a) { return a.rows * a.kv_heads * (a.head_dim / 4) > 2ll * 2048 * kvq4_sm_count(); }
+
+// Four rows a thread where one each would fill the GPU's threads more than twice over
+template <int TYPE>
+cudaError_t launch_append(cudaStream_t stream, const KvQ4Rows& a, bool vector) {
+    return many_rows(a) ? launch_rows(stream, kvq4_append_kernel<TYPE, 4>, a, 4, vector) : launch_rows(stream, kvq4_append_kernel<TYPE, 1>, a, 1, vector);
+}
+template <int TYPE>
+cudaError_t launch_read(cudaStream_t stream, const KvQ4Rows& a) {
+    return many_rows(a) ? launch_rows(stream, kvq4_read_kernel<TYPE, 4>, a, 4) : launch_rows(stream, kvq4_read_kernel<TYPE, 1>, a, 1);
+}
 
 }  // namespace
 
 cudaError_t launch_kvq4_append(cudaStream_t stream, const KvQ4Rows& a) {
     if (a.rows <= 0) return cudaSuccess;
-    const long long threads = a.rows * a.kv_heads * 2 * (a.head_dim / 8), blocks = (threads + 255) / 256;
-    if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
     const int size = a.type == kQ4F32 ? 4 : 2;
     const bool vector = aligned16(a.k, a.k_stride, size) && aligned16(a.v, a.v_stride, size);
-    if (a.type == kQ4F32) kvq4_append_kernel<kQ4F32><<<(unsigned)blocks, 256, 0, stream>>>(a, vector);
-    else if (a.type == kQ4F16) kvq4_append_kernel<kQ4F16><<<(unsigned)blocks, 256, 0, stream>>>(a, vector);
-    else kvq4_append_kernel<kQ4BF16><<<(unsigned)blocks, 256, 0, stream>>>(a, vector);
-    return cudaGetLastError();
+    return a.type == kQ4F32 ? launch_append<kQ4F32>(stream, a, vector) : a.type == kQ4F16 ? launch_append<kQ4F16>(stream, a, vector) : launch_append<kQ4BF16>(stream, a, vector);
 }
 
 cudaError_t launch_kvq4_read(cudaStream_t stream, const KvQ4Rows& a) {
     if (a.rows <= 0) return cudaSuccess;
-    const long long threads = a.rows * a.kv_heads * 2 * (a.head_dim / 8), blocks = (threads + 255) / 256;
-    if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
-    if (a.type == kQ4F32) kvq4_read_kernel<kQ4F32><<<(unsigned)blocks, 256, 0, stream>>>(a);
-    else if (a.type == kQ4F16) kvq4_read_kernel<kQ4F16><<<(unsigned)blocks, 256, 0, stream>>>(a);
-    else kvq4_read_kernel<kQ4BF16><<<(unsigned)blocks, 256, 0, stream>>>(a);
-    return cudaGetLastError();
+    return a.type == kQ4F32 ? launch_read<kQ4F32>(stream, a) : a.type == kQ4F16 ? launch_read<kQ4F16>(stream, a) : launch_read<kQ4BF16>(stream, a);
 }
 
 }  // namespace ribn

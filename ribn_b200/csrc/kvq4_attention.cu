@@ -544,6 +544,7 @@ __global__ void __launch_bounds__(kWarps * 32) kvq4_merge_kernel(const KvQ4Atten
     const int cb = id % a.col_blocks; id /= a.col_blocks;
     const int kvh = id % a.kv_heads, s = id / a.kv_heads;
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const Sequence q = sequence_of(a, s);
     if (cb >= q.blocks) return;
     const Block b = block_of(a, q, cb);
@@ -607,14 +608,14 @@ void plan_spans(KvQ4Attention& a) {
     const long long keys = a.window > 0 ? std::min<long long>(a.max_keys, (long long)a.window + a.max_rows + kQ4Page) : a.max_keys;
     const long long pages = std::max(1ll, (keys + kQ4Page - 1) / kQ4Page), items = (long long)a.sequences * a.kv_heads * a.col_blocks;
     const long long resident = (long long)kvq4_sm_count() * (a.head_dim <= 128 && a.span_cols == 8 ? (a.type == kQ4F32 ? 3 : 4) : 2);
-    a.least_pages = 3 * kWarps;
+    a.least_pages = kWarps;
     a.grid = (int)std::max(1ll, std::min(resident, (items * pages + a.least_pages - 1) / a.least_pages));
     a.max_spans = 2;   // an item may be cut, unless one CTA has all
     if (a.grid == 1) a.max_spans = 1;
 }
 
 template <typename Kernel>
-cudaError_t launch(cudaStream_t stream, Kernel kernel, long long grid, size_t smem, const KvQ4Attention& a, bool programmatic) {
+cudaError_t launch(cudaStream_t stream, Kernel kernel, long long grid, size_t smem, const KvQ4Attention& a) {
     if (grid > 0x7fffffffll) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
@@ -625,7 +626,7 @@ cudaError_t launch(cudaStream_t stream, Kernel kernel, long long grid, size_t sm
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = programmatic ? 1 : 0;
+    cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
@@ -642,7 +643,7 @@ cudaError_t launch_spans(cudaStream_t stream, const KvQ4Attention& a) {
         if (e != cudaSuccess) return e;
         configured[dev] = true;
     }
-    return launch(stream, kvq4_span_kernel<HD, NT, PAIR>, a.grid, smem, a, false);
+    return launch(stream, kvq4_span_kernel<HD, NT, PAIR>, a.grid, smem, a);
 }
 
 template <int HD>
@@ -651,7 +652,7 @@ cudaError_t launch_hd(cudaStream_t stream, const KvQ4Attention& a) {
     const bool pair = a.type == kQ4F32;
     cudaError_t e = a.span_cols == 8 ? (pair ? launch_spans<HD, 1, true>(stream, a) : launch_spans<HD, 1, false>(stream, a))
                                      : (pair ? launch_spans<HD, WIDE, true>(stream, a) : launch_spans<HD, WIDE, false>(stream, a));
-    if (e == cudaSuccess && a.max_spans > 1) e = launch(stream, kvq4_merge_kernel<HD>, (long long)a.sequences * a.kv_heads * a.col_blocks * a.merge_cols, 0, a, true);
+    if (e == cudaSuccess && a.max_spans > 1) e = launch(stream, kvq4_merge_kernel<HD>, (long long)a.sequences * a.kv_heads * a.col_blocks * a.merge_cols, 0, a);
     return e;
 }
 

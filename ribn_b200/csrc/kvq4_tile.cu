@@ -224,6 +224,8 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
     extern __shared__ __align__(128) unsigned char smem[];
     const int warp = uniform_warp(), lane = threadIdx.x & 31;
     const int group = a.q_heads / a.kv_heads, kvh = (int)blockIdx.x % a.kv_heads;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     Work w;
     if (!find_work(a, (int)blockIdx.x / a.kv_heads, lane, w)) return;
     const uint32_t at = smem_u32(smem), bars = at + T::BARS;
@@ -806,6 +808,8 @@ __global__ void __launch_bounds__(kTilePages * 32) kvq4_expand_kernel(const KvQ4
     using T = Tile<HD, false>;
     constexpr int NG = HD / 32, WORDS = NG, BLOCK = kQ4Page * 16 * WORDS, RECORD = q4_record(HD);
     const int page = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = (int)blockIdx.x % a.kv_heads, place = (int)blockIdx.x / a.kv_heads;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     int s = -1, j = 0, low = 0, high = 0, tile0 = 0;
     int before = 0;
     for (int s0 = 0; s0 < a.sequences && s < 0; s0 += 32) {   // every warp by itself
@@ -904,13 +908,24 @@ cudaError_t launch_tile(cudaStream_t stream, const KvQ4Attention& a) {
     const long long places = flats / (2 * kRows) + std::min<long long>(a.sequences, flats / (a.tile_above + 1));
     if (places * a.kv_heads > 0x7fffffffll) return cudaErrorInvalidValue;
     if (places <= 0) return cudaSuccess;
+    const auto launch = [&](auto kernel, long long grid, int threads, size_t smem) {   // early: see launch_rows
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)grid);
+        cfg.blockDim = dim3((unsigned)threads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        return cudaLaunchKernelEx(&cfg, kernel, a);
+    };
     if (a.scratch_tiles > 0) {
-        kvq4_expand_kernel<HD><<<(unsigned)(a.scratch_tiles * a.kv_heads), kTilePages * 32, 0, stream>>>(a);
-        e = cudaGetLastError();
+        e = launch(kvq4_expand_kernel<HD>, (long long)a.scratch_tiles * a.kv_heads, kTilePages * 32, 0);
         if (e != cudaSuccess) return e;
     }
-    kvq4_tile_kernel<HD, PAIR><<<(unsigned)(places * a.kv_heads), Tile<HD, PAIR>::THREADS, Tile<HD, PAIR>::SMEM, stream>>>(a);
-    return cudaGetLastError();
+    return launch(kvq4_tile_kernel<HD, PAIR>, places * a.kv_heads, Tile<HD, PAIR>::THREADS, Tile<HD, PAIR>::SMEM);
 }
 
 }  // namespace

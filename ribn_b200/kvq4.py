@@ -32,19 +32,19 @@ def _refuse(what: str):
 
 
 def _arena(cache: torch.Tensor):
-    if cache.dtype is not torch.uint8 or cache.dim() != 3 or not cache.is_contiguous() or not cache.is_cuda or cache.shape[2] % 18:
+    shape = cache.shape
+    if cache.dtype is not torch.uint8 or len(shape) != 3 or not cache.is_cuda or not cache.is_contiguous() or shape[2] % 18:
         raise ValueError("cache must be a contiguous uint8 CUDA tensor [pages][kv_heads][18 * head_dim]")
-    pages, kv_heads, record = cache.shape
-    return pages, kv_heads, record // 18, cache.device
+    return shape[0], shape[1], shape[2] // 18, cache.get_device()
 
 
-def _rows(name: str, x: torch.Tensor, heads: int, head_dim: int, device, rows: int | None = None, dtype=None):
+def _rows(name: str, x: torch.Tensor, heads: int, head_dim: int, device: int, rows: int | None = None, dtype=None):
     """A [rows][heads][head_dim] tensor whose rows are whole; the values from one row to the next."""
     shape, stride = x.shape, x.stride()
     if len(shape) != 3 or shape[1] != heads or shape[2] != head_dim or (rows is not None and shape[0] != rows):
         raise ValueError(f"{name} must be [{'rows' if rows is None else rows}][{heads}][{head_dim}]: got {list(shape)}")
-    if x.device != device or x.dtype not in _TYPES or (dtype is not None and x.dtype is not dtype):
-        raise ValueError(f"{name} must be float32, float16 or bfloat16, as its fellows are, on {device}: got {x.dtype} on {x.device}")
+    if x.get_device() != device or x.dtype not in _TYPES or (dtype is not None and x.dtype is not dtype):
+        raise ValueError(f"{name} must be float32, float16 or bfloat16, as its fellows are, on CUDA device {device}: got {x.dtype} on {x.device}")
     if shape[0] and (stride[2] != 1 or (heads > 1 and stride[1] != head_dim)):
         raise ValueError(f"{name}: the heads of a row must lie side by side")
     if shape[0] > 1 and stride[0] < heads * head_dim:
@@ -52,14 +52,16 @@ def _rows(name: str, x: torch.Tensor, heads: int, head_dim: int, device, rows: i
     return stride[0]
 
 
-def _ints(name: str, x: torch.Tensor, dims: int, device):
-    if x.dtype is not torch.int32 or x.dim() != dims or x.device != device or (x.numel() and x.stride(dims - 1) != 1):
-        raise ValueError(f"{name} must be a {dims}-dimensional int32 tensor on {device}, its last dimension contiguous")
+def _ints(name: str, x: torch.Tensor, shape: tuple, device: int):
+    """An int32 tensor of this shape whose last dimension is contiguous; its address."""
+    if x.dtype is not torch.int32 or x.shape != shape or x.get_device() != device or (x.stride()[-1] != 1 and x.numel()):
+        raise ValueError(f"{name} must be an int32 tensor of shape {list(shape)} on CUDA device {device}, its last dimension contiguous: "
+                         f"got {x.dtype} {list(x.shape)} on {x.device}")
     return x.data_ptr()
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+# the stream as a number, without a Stream object around it, which takes longer to make than a small call
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def append(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
@@ -70,10 +72,8 @@ def append(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.T
     k_stride = _rows("k", k, kv_heads, head_dim, device)
     rows = k.shape[0]
     v_stride = _rows("v", v, kv_heads, head_dim, device, rows, k.dtype)
-    at = _ints("slots", slots, 1, device)
-    if slots.shape[0] != rows:
-        raise ValueError("slots must name one slot per row")
-    if lib().ribn_b200_kvq4_append(device.index, _stream(device), cache.data_ptr(), pages, kv_heads, head_dim, _TYPES[k.dtype], k.data_ptr(),
+    at = _ints("slots", slots, (rows,), device)
+    if lib().ribn_b200_kvq4_append(device, _raw_stream(device), cache.data_ptr(), pages, kv_heads, head_dim, _TYPES[k.dtype], k.data_ptr(),
                                    k_stride, v.data_ptr(), v_stride, at, rows) != OK:
         _refuse("kvq4_append")
 
@@ -82,12 +82,13 @@ def read(cache: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = torch.fl
     """(k, v) [rows][kv_heads][head_dim]: the cached values at slots[row], which float16 and float32 hold exactly; zeros where a slot
     lies outside of the arena."""
     pages, kv_heads, head_dim, device = _arena(cache)
-    at = _ints("slots", slots, 1, device)
+    rows = slots.shape[0] if slots.dim() == 1 else -1
+    at = _ints("slots", slots, (rows,), device)
     if dtype not in _TYPES:
         raise ValueError("dtype must be float32, float16 or bfloat16")
-    rows = slots.shape[0]
-    k, v = torch.empty((2, rows, kv_heads, head_dim), dtype=dtype, device=device).unbind(0)
-    if lib().ribn_b200_kvq4_read(device.index, _stream(device), cache.data_ptr(), pages, kv_heads, head_dim, _TYPES[dtype], at, rows,
+    shape = (rows, kv_heads, head_dim)
+    k, v = torch.empty(shape, dtype=dtype, device=cache.device), torch.empty(shape, dtype=dtype, device=cache.device)
+    if lib().ribn_b200_kvq4_read(device, _raw_stream(device), cache.data_ptr(), pages, kv_heads, head_dim, _TYPES[dtype], at, rows,
                                  k.data_ptr(), v.data_ptr()) != OK:
         _refuse("kvq4_read")
     return k, v
@@ -107,23 +108,24 @@ def attention(cache: torch.Tensor, q: torch.Tensor, page_tables: torch.Tensor, l
         raise ValueError(f"q must be [rows][q_heads][{head_dim}], q_heads a multiple of the cache's {kv_heads}")
     rows, q_heads, _ = q.shape
     q_stride = _rows("q", q, q_heads, head_dim, device)
-    sequences = lengths.shape[0] if lengths.dim() == 1 else -1
-    tables, at_lengths, at_rows = _ints("page_tables", page_tables, 2, device), _ints("lengths", lengths, 1, device), _ints("cu_rows", cu_rows, 1, device)
-    if page_tables.shape[0] != sequences or cu_rows.shape[0] != sequences + 1:
-        raise ValueError("page_tables, lengths and cu_rows must have sequences, sequences and sequences + 1 rows")
+    if page_tables.dim() != 2:
+        raise ValueError("page_tables must be [sequences][pages of the longest]")
+    sequences, width = page_tables.shape
+    tables, at_lengths = _ints("page_tables", page_tables, (sequences, width), device), _ints("lengths", lengths, (sequences,), device)
+    at_rows = _ints("cu_rows", cu_rows, (sequences + 1,), device)
     if scale is not None and not 0.0 < abs(scale) < float("inf"):
         raise ValueError("scale must be finite and not zero")
     if out is None:
-        out = torch.zeros((rows, q_heads, head_dim), dtype=q.dtype, device=device)
+        out = torch.zeros((rows, q_heads, head_dim), dtype=q.dtype, device=q.device)
     out_stride = _rows("out", out, q_heads, head_dim, device, rows, q.dtype)
     args = KvQ4AttentionArgs(cache.data_ptr(), pages, q.data_ptr(), out.data_ptr(), tables, at_lengths, at_rows, None, 0, q_stride, out_stride,
-                             page_tables.stride(0), _TYPES[q.dtype], q_heads, kv_heads, head_dim, page_tables.shape[1], sequences, rows,
+                             page_tables.stride(0), _TYPES[q.dtype], q_heads, kv_heads, head_dim, width, sequences, rows,
                              min(max_rows, rows), max_keys, window, scale or 0.0, 0)
     library = lib()
     need = library.ribn_b200_kvq4_workspace(args)
     if need:
-        scratch = torch.empty(need, dtype=torch.uint8, device=device)
+        scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
         args.workspace, args.workspace_bytes = scratch.data_ptr(), need
-    if library.ribn_b200_kvq4_attention(device.index, _stream(device), args) != OK:
+    if library.ribn_b200_kvq4_attention(device, _raw_stream(device), args) != OK:
         _refuse("kvq4_attention")
     return out
