@@ -60,6 +60,8 @@ struct KvQ4Attention {
     long long* prefix;                 // pages of the span kernel's list before each sequence, and of all
     unsigned char* scratch;            // operands of the tile kernel's key tiles, [tile][kv_head][512 head_dim bytes]
     int scratch_tiles;                 // how many tiles there is room for
+    int tile_splits;                   // CTAs that share a pair of query tiles' keys, their sums in tile_partial, [row][q_head][split][head_dim + 4]
+    float* tile_partial;
     int tile_above;                    // a sequence with more query rows (rows x heads of a group) than this takes the tile kernel
 };
 // Bytes of scratch that launch_kvq4_attention can use; it works with less than the tile kernel's part, not with less than the sums.
@@ -68,6 +70,8 @@ cudaError_t launch_kvq4_attention(cudaStream_t stream, KvQ4Attention a);
 
 // The sequences with more than `tile_above` query rows (kvq4_tile.cu; heads of 64 and 128).
 cudaError_t launch_kvq4_tiles(cudaStream_t stream, const KvQ4Attention& a);
+// At most this many pairs of its query tiles, however the rows are spread over the sequences.
+long long kvq4_tile_places(const KvQ4Attention& a);
 
 int kvq4_sm_count();
 

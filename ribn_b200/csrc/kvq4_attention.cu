@@ -676,12 +676,24 @@ size_t partial_bytes(const KvQ4Attention& a) {
     const size_t n = a.max_spans > 1 ? prefix_bytes(a) + (size_t)a.grid * 2 * a.span_cols * (a.head_dim + 2) * sizeof(float) : 0;
     return (n + 255) / 256 * 256;
 }
+bool has_tiles(const KvQ4Attention& a) { return (long long)std::min(a.max_rows, a.rows) * (a.q_heads / a.kv_heads) > a.tile_above; }
+long long seen_keys(const KvQ4Attention& a) { return a.window > 0 ? std::min<long long>(a.max_keys, (long long)a.window + a.max_rows) : a.max_keys; }
 int wanted_tiles(const KvQ4Attention& a) {
+    if (!has_tiles(a)) return 0;
     const long long flats = (long long)a.rows * (a.q_heads / a.kv_heads);
-    if ((long long)std::min(a.max_rows, a.rows) * (a.q_heads / a.kv_heads) <= a.tile_above) return 0;
-    const long long keys = a.window > 0 ? std::min<long long>(a.max_keys, (long long)a.window + a.max_rows) : a.max_keys;
-    const long long tiles = std::min<long long>(a.sequences, flats / (a.tile_above + 1)) * (keys / 128 + 2), room = (long long)(kScratchMost / ((size_t)512 * a.head_dim * a.kv_heads));
+    const long long tiles = std::min<long long>(a.sequences, flats / (a.tile_above + 1)) * (seen_keys(a) / 128 + 2), room = (long long)(kScratchMost / ((size_t)512 * a.head_dim * a.kv_heads));
     return (int)std::min(tiles, room);
+}
+// While query tiles leave SMs idle their keys are shared, two key tiles to a CTA at least: 16 rows behind 8,000 keys, 32 / 8 heads, 182 us
+// without.  The sums of rows x q_heads x splits are those of at most 256 rows per SM.
+int wanted_splits(const KvQ4Attention& a) {
+    if (!has_tiles(a)) return 1;
+    const long long ctas = std::max(1ll, kvq4_tile_places(a) * a.kv_heads), tiles = std::max(1ll, seen_keys(a) / 128 + 1);
+    return (int)std::max(1ll, std::min(kvq4_sm_count() / ctas, (tiles + 1) / 2));
+}
+size_t split_bytes(const KvQ4Attention& a) {
+    const int splits = wanted_splits(a);
+    return splits > 1 ? (size_t)a.rows * a.q_heads * splits * (a.head_dim + 4) * sizeof(float) : 0;
 }
 
 }  // namespace
@@ -689,17 +701,19 @@ int wanted_tiles(const KvQ4Attention& a) {
 size_t kvq4_workspace_bytes(const KvQ4Attention& args) {
     KvQ4Attention a = args;
     plan_spans(a);
-    return partial_bytes(a) + (size_t)wanted_tiles(a) * 512 * a.head_dim * a.kv_heads;
+    return partial_bytes(a) + split_bytes(a) + (size_t)wanted_tiles(a) * 512 * a.head_dim * a.kv_heads;
 }
 
 cudaError_t launch_kvq4_attention(cudaStream_t stream, KvQ4Attention a) {
     if (a.rows <= 0 || a.sequences <= 0) return cudaSuccess;
     plan_spans(a);
-    const size_t sums = partial_bytes(a);
+    const size_t runs = partial_bytes(a), sums = runs + split_bytes(a);
     if (a.partial_bytes < sums) return cudaErrorInvalidValue;
+    a.tile_splits = wanted_splits(a);
     unsigned char* scratch = reinterpret_cast<unsigned char*>(a.partial);
     a.prefix = reinterpret_cast<long long*>(scratch);
     a.partial = reinterpret_cast<float*>(scratch + prefix_bytes(a));
+    a.tile_partial = reinterpret_cast<float*>(scratch + runs);
     a.scratch = scratch + sums;
     a.scratch_tiles = (int)std::min<size_t>((size_t)wanted_tiles(a), (a.partial_bytes - sums) / ((size_t)512 * a.head_dim * a.kv_heads));
     const int size = a.type == kQ4F32 ? 4 : 2;

@@ -227,7 +227,8 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     Work w;
-    if (!find_work(a, (int)blockIdx.x / a.kv_heads, lane, w)) return;
+    const int split = (int)blockIdx.x / a.kv_heads % a.tile_splits;
+    if (!find_work(a, (int)blockIdx.x / a.kv_heads / a.tile_splits, lane, w)) return;
     const uint32_t at = smem_u32(smem), bars = at + T::BARS;
     const uint32_t q_full = bars, s_full = bars + 16, p_full = bars + 32, o_full = bars + 48, k_full = bars + 64, k_empty = bars + 80, v_full = bars + 96, v_empty = bars + 112,
                    drained = bars + 128, tmem_slot = bars + 144, failed = bars + 148;
@@ -251,7 +252,8 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
 
     // a tile's rows and key tiles; key tiles begin at multiples of 128, the first one where the pair's first row looks
     int live[2], n[2];
-    const int low = a.window > 0 ? max(0, w.base + w.flat0 / group - a.window + 1) : 0, first_tile = low / kKeys;
+    const int low = a.window > 0 ? max(0, w.base + w.flat0 / group - a.window + 1) : 0;
+    int first_tile = low / kKeys;
     int high = 0;
     for (int t = 0; t < 2; ++t) {
         const int flat = w.flat0 + t * kRows;
@@ -260,6 +262,12 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
         n[t] = max(0, (to + kKeys - 1) / kKeys - first_tile);
         if (to <= 0) n[t] = 0;
         high = max(high, to);
+    }
+    {   // this CTA's share of them
+        const int share = (max(n[0], n[1]) + a.tile_splits - 1) / a.tile_splits, begin = split * share;
+        first_tile += begin;
+        n[0] = max(0, min(n[0] - begin, share));
+        n[1] = max(0, min(n[1] - begin, share));
     }
     const int n_tiles = max(n[0], n[1]);
     // the sequence's keys as operands in memory, where the call has room for them
@@ -517,18 +525,27 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
         if (own > 0) {
             // the warp's 32 query rows: lane = (row of eight, 8-dimension piece of four), scaled so that a row's largest lies in [2^13, 2^14)
             const int sub = lane & 7, pc = lane >> 3;
-            constexpr int PP = HD / 32;   // pieces per lane and row
-#pragma unroll 1
-            for (int rg = 4 / HALVES * part; rg < 4 / HALVES * (part + 1); ++rg) {
-                const int r = row0 + rg * 8 + sub;
-                float x[PP][8], top = 0.0f;
+            constexpr int PP = HD / 32, GROUPS = 4 / HALVES;   // pieces per lane and row; groups of eight rows
+            uint32_t raw[GROUPS][PP][PAIR ? 8 : 4];            // everything in flight together
+#pragma unroll
+            for (int i = 0; i < GROUPS; ++i) {
+                const int r = row0 + (GROUPS * part + i) * 8 + sub;
 #pragma unroll
                 for (int p = 0; p < PP; ++p) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x[p][i] = 0.0f;
-                    if (r < live_rows) q4_load8<PAIR>(a.q, (w.row0 + (flat0 + r) / group) * a.q_stride + (long long)(kvh * group + (flat0 + r) % group) * HD + (p * 4 + pc) * 8, a.type, a.vector_q, x[p]);
+                    for (int u = 0; u < (PAIR ? 8 : 4); ++u) raw[i][p][u] = 0u;
+                    if (r < live_rows) q4_load_raw(a.q, (w.row0 + (flat0 + r) / group) * a.q_stride + (long long)(kvh * group + (flat0 + r) % group) * HD + (p * 4 + pc) * 8, a.vector_q, raw[i][p]);
+                }
+            }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[p][i]));
+            for (int i = 0; i < GROUPS; ++i) {
+                const int rg = GROUPS * part + i, r = row0 + rg * 8 + sub;
+                float x[PP][8], top = 0.0f;
+#pragma unroll
+                for (int p = 0; p < PP; ++p) {
+                    q4_values(raw[i][p], a.type, x[p]);
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) top = fmaxf(top, fabsf(x[p][u]));
                 }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -734,6 +751,14 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
                 const float other = __uint_as_float(lds32(other_at));
                 total = part == 0 ? total + other : other + total;
             }
+            // where the keys are shared with other CTAs: the row's sums, for the merge
+            const bool shared = a.tile_splits > 1, have_row = row < live_rows;
+            float* record = a.tile_partial + (((long long)(w.row0 + (flat0 + row) / group) * a.q_heads + kvh * group + (flat0 + row) % group) * a.tile_splits + split) * (HD + 4);
+            if (shared && have_row && part == 0) {
+                const bool none = own == 0 || (!PAIR && m == kUnset) || (PAIR && m == -INFINITY);
+                record[HD] = !alive || lds32(failed) != 0 ? __int_as_float(0x7fffffff) : none && total == total ? -INFINITY : PAIR ? m * factor : m;
+                record[HD + 1] = total;
+            }
             const uint32_t stage = q_tile + ((warp & 3) * HALVES + part) * 32 * ROW_BYTES;
             float inv = total > 0.0f ? 1.0f / total : total != total ? total : 0.0f;
             if (!alive || lds32(failed) != 0) inv = __int_as_float(0x7fffffff);
@@ -747,7 +772,14 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
 #pragma unroll
                     for (int u = 0; u < 32; ++u) {
                         if (PAIR) o[u] = fmaf(sum[PAIR ? i + u : 0], since, o[u]);
-                        o[u] = inv != 0.0f ? o[u] * inv : 0.0f;
+                        if (!shared) o[u] = inv != 0.0f ? o[u] * inv : 0.0f;
+                    }
+                    if (shared) {
+#pragma unroll
+                        for (int u = 0; u < 32; u += 4) {
+                            if (have_row) *reinterpret_cast<float4*>(record + part * DH + i + u) = make_float4(o[u], o[u + 1], o[u + 2], o[u + 3]);
+                        }
+                        continue;
                     }
 #pragma unroll
                     for (int u = 0; u < 32; u += 16 / VALUE) {
@@ -772,7 +804,7 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
             __syncwarp();
             constexpr int PER = 32 / PIECES;   // rows per pass
 #pragma unroll 1
-            for (int r0 = 0; r0 < 32; r0 += PER) {
+            for (int r0 = 0; r0 < 32 && !shared; r0 += PER) {
                 const int r = r0 + lane / PIECES, p = lane % PIECES, flat = flat0 + row0 + r;
                 if (row0 + r >= live_rows) continue;
                 const uint4 v = lds128(stage + r * ROW_BYTES + ((p ^ (r & SWAP)) << 4));
@@ -799,6 +831,49 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
     if (warp == T::MMA_WARP) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// A row's sums over its key tiles' shares: out = sum_s acc_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), shares in order, a warp per (row, query head).
+template <int HD>
+__global__ void __launch_bounds__(128) kvq4_tile_merge_kernel(const KvQ4Attention a) {
+    constexpr int PER = HD / 32;
+    const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, row = (int)(id / a.q_heads), qh = (int)(id % a.q_heads), group = a.q_heads / a.kv_heads;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (row >= a.rows) return;
+    int s = 0, above = a.sequences;   // the last sequence that begins at or before the row
+    while (above - s > 1) {
+        const int mid = (s + above) / 2;
+        if (a.cu_rows[mid] <= row) s = mid; else above = mid;
+    }
+    const int row0 = max(a.cu_rows[s], 0), n = min(min(a.cu_rows[s + 1], a.rows) - row0, a.max_rows);
+    if (row < row0 || row >= row0 + n || (long long)n * group <= a.tile_above) return;   // not the tile kernel's
+    const float* from = a.tile_partial + id * a.tile_splits * (HD + 4);
+    float top = -INFINITY;
+    for (int i = lane; i < a.tile_splits; i += 32) top = fmaxf(top, __ldcg(from + (long long)i * (HD + 4) + HD));
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    float sum[PER], total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sum[i] = 0.0f;
+    for (int i = 0; i < a.tile_splits; ++i) {
+        const float* rec = from + (long long)i * (HD + 4);
+        const float m = __ldcg(rec + HD);
+        if (m == -INFINITY) continue;   // no key: its values were not written
+        const float f = exp2_approx(m - top);
+        total = fmaf(__ldcg(rec + HD + 1), f, total);
+#pragma unroll
+        for (int u = 0; u < PER; ++u) sum[u] = fmaf(__ldcg(rec + lane + 32 * u), f, sum[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+        const float x = total > 0.0f || total != total ? sum[u] / total : 0.0f;
+        const long long to = row * a.out_stride + (long long)qh * HD + lane + 32 * u;
+        if (a.type == kQ4F32) static_cast<float*>(a.out)[to] = x;
+        else if (a.type == kQ4F16) static_cast<__half*>(a.out)[to] = __float2half_rn(x);
+        else asm volatile("{\n\t.reg .b16 t;\n\tcvt.rn.bf16.f32 t, %1;\n\tst.global.b16 [%0], t;\n\t}" ::"l"(static_cast<unsigned short*>(a.out) + to), "f"(x) : "memory");
     }
 }
 
@@ -892,7 +967,7 @@ __global__ void __launch_bounds__(kTilePages * 32) kvq4_expand_kernel(const KvQ4
 }
 
 template <int HD, bool PAIR>
-cudaError_t launch_tile(cudaStream_t stream, const KvQ4Attention& a) {
+cudaError_t launch_tile(cudaStream_t stream, KvQ4Attention a) {
     static bool configured[kMaxDevices] = {false};   // function attributes are per device
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -904,9 +979,8 @@ cudaError_t launch_tile(cudaStream_t stream, const KvQ4Attention& a) {
         configured[dev] = true;
     }
     // at most this many pairs of tiles, however the rows are spread over the sequences
-    const long long flats = (long long)a.rows * (a.q_heads / a.kv_heads);
-    const long long places = flats / (2 * kRows) + std::min<long long>(a.sequences, flats / (a.tile_above + 1));
-    if (places * a.kv_heads > 0x7fffffffll) return cudaErrorInvalidValue;
+    const long long places = kvq4_tile_places(a);
+    if (places * a.tile_splits * a.kv_heads > 0x7fffffffll) return cudaErrorInvalidValue;
     if (places <= 0) return cudaSuccess;
     const auto launch = [&](auto kernel, long long grid, int threads, size_t smem) {   // early: see launch_rows
         cudaLaunchConfig_t cfg = {};
@@ -925,10 +999,17 @@ cudaError_t launch_tile(cudaStream_t stream, const KvQ4Attention& a) {
         e = launch(kvq4_expand_kernel<HD>, (long long)a.scratch_tiles * a.kv_heads, kTilePages * 32, 0);
         if (e != cudaSuccess) return e;
     }
-    return launch(kvq4_tile_kernel<HD, PAIR>, places * a.kv_heads, Tile<HD, PAIR>::THREADS, Tile<HD, PAIR>::SMEM);
+    e = launch(kvq4_tile_kernel<HD, PAIR>, places * a.tile_splits * a.kv_heads, Tile<HD, PAIR>::THREADS, Tile<HD, PAIR>::SMEM);
+    if (e == cudaSuccess && a.tile_splits > 1) e = launch(kvq4_tile_merge_kernel<HD>, ((long long)a.rows * a.q_heads + 3) / 4, 128, 0);
+    return e;
 }
 
 }  // namespace
+
+long long kvq4_tile_places(const KvQ4Attention& a) {
+    const long long flats = (long long)a.rows * (a.q_heads / a.kv_heads);
+    return flats / (2 * kRows) + std::min<long long>(a.sequences, flats / (a.tile_above + 1));
+}
 
 cudaError_t launch_kvq4_tiles(cudaStream_t stream, const KvQ4Attention& a) {
     const bool pair = a.type == kQ4F32;
