@@ -463,7 +463,7 @@ RIBN_B200_API int ribn_b200_attention_noalloc(int32_t device, void* stream, cons
  * head, a binary16 scale, 4.5 bits together.  A value is scale x (code - 8), exact in binary16.  The byte order is the
  * kernels' own; a zeroed arena holds zeros.  Every pointer is a DEVICE pointer, work is enqueued on `stream` (a cudaStream_t)
  * with `device` current (the caller's current device is restored), nothing is allocated and nothing waits, so the calls may be
- * captured into a graph.  Refusals return RIBN_B200_ERROR with a message in ribn_b200_op_last_error and enqueue nothing.
+ * captured into a graph (make one call of the kind before, which loads its kernels).  Refusals return RIBN_B200_ERROR with a message in ribn_b200_op_last_error and enqueue nothing.
  * `type` is that of the rows: RIBN_B200_KVQ4_F32, _F16 or _BF16. */
 enum { RIBN_B200_KVQ4_F32 = 0, RIBN_B200_KVQ4_F16 = 1, RIBN_B200_KVQ4_BF16 = 2 };
 /* Quantises rows k, v `[rows][kv_heads][head_dim]` (`k_stride`, `v_stride`: values from one row to the next) into the arena at
@@ -484,8 +484,9 @@ RIBN_B200_API int ribn_b200_kvq4_read(int32_t device, void* stream, const void* 
  * window > 0 the last `window` of those.  A row that sees no key (its position is negative) gets zeros; rows of q that no
  * sequence has are left alone in `out`; a page number outside of the arena hides its keys.  `max_rows` bounds the rows of
  * a sequence (later ones are left alone); `max_keys` sets how the work is split, results are right for any.  `scale` 0 is
- * 1 / sqrt(head_dim).  `q_stride`, `out_stride`: values from one row to the next.  `workspace` (16-byte aligned, what
- * ribn_b200_kvq4_workspace asks for) is scratch of this call: calls that may overlap on the GPU, or graphs that may replay
+ * 1 / sqrt(head_dim).  `q_stride`, `out_stride`: values from one row to the next; `out` does not overlap `q`.  At most 2^26 pages
+ * per sequence.  `workspace` (16-byte aligned, what ribn_b200_kvq4_workspace asks for; the part that it asks for operands of
+ * sequences with many rows may be missing, which is slower) is scratch of this call: calls that may overlap on the GPU, or graphs that may replay
  * at once, need one each. */
 typedef struct {
     const void* cache;

@@ -52,7 +52,8 @@ KvQ4Attention attention_of(const ribn_b200_kvq4_attention_args& x) {
     a.q = x.q; a.q_stride = x.q_stride; a.out_stride = x.out_stride; a.out = x.out;
     a.page_tables = x.page_tables; a.pages_per_sequence = x.pages_per_sequence; a.table_stride = x.table_stride;
     a.lengths = x.lengths; a.cu_rows = x.cu_rows;
-    a.sequences = x.sequences; a.rows = x.rows; a.max_rows = x.max_rows; a.max_keys = x.max_keys; a.window = x.window;
+    a.sequences = x.sequences; a.rows = x.rows; a.max_rows = x.max_rows; a.max_keys = x.max_keys;
+    a.window = x.window >= x.pages_per_sequence * kQ4Page ? 0 : x.window;   // over everything a sequence can have: none
     a.scale = x.scale == 0.0f ? 1.0f / sqrtf((float)x.head_dim) : x.scale;
     a.partial = static_cast<float*>(x.workspace); a.partial_bytes = x.workspace_bytes;
     return a;
@@ -65,7 +66,7 @@ const char* bad_attention(const ribn_b200_kvq4_attention_args& a) {
     }
     if (a.head_dim != 64 && a.head_dim != 128 && a.head_dim != 256) return "kvq4: head_dim must be 64, 128 or 256";
     if (a.rows < 0 || a.sequences < 0 || a.max_rows < 0 || a.max_keys < 0 || a.window < 0 || a.pages_per_sequence < 0) return "kvq4_attention: negative size";
-    if ((int64_t)a.rows * a.q_heads > INT32_MAX || a.pages_per_sequence > INT32_MAX / kQ4Page || a.max_keys > INT32_MAX - kQ4Page || a.max_rows > a.rows) {
+    if ((int64_t)a.rows * a.q_heads > INT32_MAX || a.pages_per_sequence > (1 << 26) || a.max_keys > INT32_MAX - kQ4Page || a.max_rows > a.rows) {
         return "kvq4_attention: rows x q_heads, pages_per_sequence or max_keys too large, or max_rows over rows";
     }
     return nullptr;

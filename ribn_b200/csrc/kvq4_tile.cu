@@ -39,7 +39,7 @@ constexpr int kTilePages = kKeys / kQ4Page;
 constexpr uint32_t kSpinLimit = 1u << 22;
 constexpr float kLog2e = 1.4426950408889634f, kHeld = 7.0f, kSlack = 8.0f;
 constexpr int kPolynomial = 4;   // of 16 pairs of probabilities: those whose exponentials the multiply-add pipe computes
-constexpr float kUnset = -1e30f;
+constexpr float kUnset = -3e38f;   // below every finite score's place
 constexpr int kWindow = 2;   // PAIR: key tiles whose products one sum in tensor memory holds
 
 template <int HD, bool PAIR>
@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
                     if (moves) m = mx;
                     rescale(f);
                 }
-                const float shift = m == -INFINITY ? 0.0f : kHeld - m * factor;
+                const float shift = m == -INFINITY ? 0.0f : kHeld - __fmul_rn(m, factor);
 #pragma unroll 1
                 for (int i = 0; i < kKeys; i += 32) {
                     tmem_ld32(s_at + i, s);
@@ -669,7 +669,8 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
                     uint32_t hi[16], lo[16];
 #pragma unroll
                     for (int u = 0; u < 16; ++u) {
-                        const float2 y = __ffma2_rn(make_float2(s[2 * u], s[2 * u + 1]), make_float2(factor, factor), make_float2(shift, shift));
+                        // (rounded before the reference is taken off, as the reference is: the largest score's difference is zero however large)
+                        const float2 y = __fadd2_rn(make_float2(__fmul_rn(s[2 * u], factor), __fmul_rn(s[2 * u + 1], factor)), make_float2(shift, shift));
                         const float2 p = make_float2(exp2_approx(y.x), exp2_approx(y.y));
                         l = __fadd2_rn(l, p);
                         split2(p.x, p.y, hi[u], lo[u]);
@@ -691,13 +692,20 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
                         tmem_ld32(s_at + i, s);
                         const float shift = kHeld - m;
                         l0 = l1 = 0.0f;
+                        // so large that a fused multiply-add's exact product is far from the reference, a rounded one: round first
+                        const bool large = __any_sync(0xffffffffu, fabsf(m) > 4194304.0f && m != kUnset);
+                        const float times = large ? 1.0f : factor;
                         tmem_wait_ld();
                         tmem_tie32(s);
                         if (masked) hide(s, i);
-                        mx = most_of(s) * factor;
+                        if (large) {
+#pragma unroll
+                            for (int u = 0; u < 32; ++u) s[u] *= factor;
+                        }
+                        mx = most_of(s) * times;
 #pragma unroll
                         for (int u = 0; u < 16; ++u) {
-                            const float2 y = __ffma2_rn(make_float2(s[2 * u], s[2 * u + 1]), make_float2(factor, factor), make_float2(shift, shift));
+                            const float2 y = __ffma2_rn(make_float2(s[2 * u], s[2 * u + 1]), make_float2(times, times), make_float2(shift, shift));
                             const float2 p = (u * kPolynomial) % 16 < kPolynomial ? exp2_pair(y) : make_float2(exp2_approx(y.x), exp2_approx(y.y));
                             const float2 lp = __fadd2_rn(make_float2(l0, l1), p);
                             l0 = lp.x;
@@ -756,7 +764,7 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
             float* record = a.tile_partial + (((long long)(w.row0 + (flat0 + row) / group) * a.q_heads + kvh * group + (flat0 + row) % group) * a.tile_splits + split) * (HD + 4);
             if (shared && have_row && part == 0) {
                 const bool none = own == 0 || (!PAIR && m == kUnset) || (PAIR && m == -INFINITY);
-                record[HD] = !alive || lds32(failed) != 0 ? __int_as_float(0x7fffffff) : none && total == total ? -INFINITY : PAIR ? m * factor : m;
+                record[HD] = !alive || lds32(failed) != 0 ? __int_as_float(0x7fffffff) : none && total == total ? -INFINITY : PAIR ? __fmul_rn(m, factor) : m;
                 record[HD + 1] = total;
             }
             const uint32_t stage = q_tile + ((warp & 3) * HALVES + part) * 32 * ROW_BYTES;
