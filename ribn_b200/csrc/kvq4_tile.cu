@@ -159,10 +159,11 @@ struct Tiles {
     int first, count, tile0, low, high;   // keys low <= key < high are seen by some row
 };
 __device__ __forceinline__ int tiles_of(const KvQ4Attention& a, int s, int& tile0, int& low, int& high) {
-    const int group = a.q_heads / a.kv_heads, row0 = max(a.cu_rows[s], 0), all = min(a.cu_rows[s + 1], a.rows) - row0, n = min(all, a.max_rows);
+    const int group = a.q_heads / a.kv_heads, begin = a.cu_rows[s], end = a.cu_rows[s + 1], length = a.lengths[s];
+    const int row0 = max(begin, 0), all = min(end, a.rows) - row0, n = min(all, a.max_rows);
     tile0 = low = high = 0;
     if (n <= 0 || (long long)n * group <= a.tile_above) return 0;
-    const int base = min(max(a.lengths[s], 0), a.pages_per_sequence * kQ4Page) - all;
+    const int base = min(max(length, 0), a.pages_per_sequence * kQ4Page) - all;
     high = max(0, base + n);
     low = a.window > 0 ? max(0, base - a.window + 1) : 0;
     tile0 = low / kKeys;
@@ -188,10 +189,13 @@ __device__ __forceinline__ bool find_work(const KvQ4Attention& a, int place, int
     const int group = a.q_heads / a.kv_heads;
     for (int s0 = 0; s0 < a.sequences; s0 += 32) {
         const int s = s0 + lane;
-        int n = 0, row0 = 0;
-        if (s < a.sequences) {
-            row0 = max(a.cu_rows[s], 0);
-            n = min(min(a.cu_rows[s + 1], a.rows) - row0, a.max_rows);
+        int n = 0, row0 = 0, base = 0;
+        if (s < a.sequences) {   // (the three loads together: one after the other they were a third of a small call)
+            const int begin = a.cu_rows[s], end = a.cu_rows[s + 1], length = a.lengths[s];
+            row0 = max(begin, 0);
+            const int all = min(end, a.rows) - row0;
+            n = min(all, a.max_rows);
+            base = min(max(length, 0), a.pages_per_sequence * kQ4Page) - all;   // `n` is cut at max_rows
         }
         const int mine = n > 0 && (long long)n * group > a.tile_above ? (n * group + 2 * kRows - 1) / (2 * kRows) : 0;
         int before = mine;
@@ -208,8 +212,7 @@ __device__ __forceinline__ bool find_work(const KvQ4Attention& a, int place, int
             w.n = __shfl_sync(0xffffffffu, n, at);
             const int pairs = __shfl_sync(0xffffffffu, mine, at), first = __shfl_sync(0xffffffffu, before, at) - pairs;
             w.flat0 = (pairs - 1 - (place - first)) * 2 * kRows;
-            const int all = min(a.cu_rows[w.s + 1], a.rows) - w.row0;   // `n` is cut at max_rows
-            w.base = min(max(a.lengths[w.s], 0), a.pages_per_sequence * kQ4Page) - all;
+            w.base = __shfl_sync(0xffffffffu, base, at);
             return true;
         }
         place -= __shfl_sync(0xffffffffu, before, 31);
@@ -525,32 +528,34 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
         if (own > 0) {
             // the warp's 32 query rows: lane = (row of eight, 8-dimension piece of four), scaled so that a row's largest lies in [2^13, 2^14)
             const int sub = lane & 7, pc = lane >> 3;
-            constexpr int PP = HD / 32, GROUPS = 4 / HALVES;   // pieces per lane and row; groups of eight rows
-            uint32_t raw[GROUPS][PP][PAIR ? 8 : 4];            // everything in flight together
-#pragma unroll
-            for (int i = 0; i < GROUPS; ++i) {
-                const int r = row0 + (GROUPS * part + i) * 8 + sub;
+            constexpr int PP = HD / 32, GROUPS = 4 / HALVES, WORDS8 = PAIR ? 8 : 4;   // pieces per lane and row; groups of eight rows
+            uint32_t next[PP][WORDS8];   // (a loop, the next group's loads under this one's arithmetic: straight code is fetched as slowly as data)
+            auto ask = [&](int rg) {
+                const int r = row0 + rg * 8 + sub;
+                const long long from = (w.row0 + (flat0 + r) / group) * a.q_stride + (long long)(kvh * group + (flat0 + r) % group) * HD + pc * 8;
 #pragma unroll
                 for (int p = 0; p < PP; ++p) {
 #pragma unroll
-                    for (int u = 0; u < (PAIR ? 8 : 4); ++u) raw[i][p][u] = 0u;
-                    if (r < live_rows) q4_load_raw(a.q, (w.row0 + (flat0 + r) / group) * a.q_stride + (long long)(kvh * group + (flat0 + r) % group) * HD + (p * 4 + pc) * 8, a.vector_q, raw[i][p]);
+                    for (int u = 0; u < WORDS8; ++u) next[p][u] = 0u;
+                    if (r < live_rows) q4_load_raw(a.q, from + p * 32, a.vector_q, next[p]);
                 }
-            }
-#pragma unroll
-            for (int i = 0; i < GROUPS; ++i) {
-                const int rg = GROUPS * part + i, r = row0 + rg * 8 + sub;
+            };
+            ask(GROUPS * part);
+#pragma unroll 1
+            for (int rg = GROUPS * part; rg < GROUPS * (part + 1); ++rg) {
+                const int r = row0 + rg * 8 + sub;
                 float x[PP][8], top = 0.0f;
 #pragma unroll
                 for (int p = 0; p < PP; ++p) {
-                    q4_values(raw[i][p], a.type, x[p]);
+                    q4_values(next[p], a.type, x[p]);
 #pragma unroll
                     for (int u = 0; u < 8; ++u) top = fmaxf(top, fabsf(x[p][u]));
                 }
+                if (rg + 1 < GROUPS * (part + 1)) ask(rg + 1);
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
                 const int e = top > 0.0f && top < INFINITY ? max(-126, min(126, 140 - (int)(__float_as_uint(top) >> 23))) : 0;
-                const float up = __int_as_float((e + 127) << 23), f = __int_as_float((127 - e) << 23), sign = a.scale < 0.0f ? -1.0f : 1.0f;
+                const float up = __int_as_float((e + 127) << 23) * (a.scale < 0.0f ? -1.0f : 1.0f), f = __int_as_float((127 - e) << 23);
                 const float scaled = f * (fabsf(a.scale) * kLog2e);
                 if constexpr (HALVES == 1) {
                     const float of_row = __shfl_sync(0xffffffffu, scaled, lane & 7);
@@ -563,7 +568,10 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
                     uint4 hi, lo;
                     uint32_t *h = &hi.x, *l = &lo.x;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) split2(x[p][i] * up * sign, x[p][i + 4] * up * sign, h[i], l[i]);
+                    for (int i = 0; i < 4; ++i) {
+                        if (PAIR) split2(x[p][i] * up, x[p][i + 4] * up, h[i], l[i]);
+                        else h[i] = as_bits(__floats2half2_rn(x[p][i] * up, x[p][i + 4] * up));
+                    }
                     const uint32_t to = q_tile + (p * 4 + pc) * T::Q_STRIDE + r * 16;
                     sts128(to, hi);
                     if (PAIR) sts128(to + T::Q_TILE, lo);
@@ -679,6 +687,24 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
                     tmem_st16(s_at + i + 16, lo);
                 }
             } else {
+                if (j == 0) {   // the first reference, from the first scores
+                    float mx = -INFINITY;
+#pragma unroll 1
+                    for (int i = 64 * part; i < 64 * part + 64; i += 32) {
+                        float s[32];
+                        tmem_ld32(s_at + i, s);
+                        tmem_wait_ld();
+                        tmem_tie32(s);
+                        if (masked) hide(s, i);
+                        mx = fmaxf(mx, most_of(s));
+                    }
+                    mx *= factor;
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine_at), "f"(mx) : "memory");
+                    pair_sync();
+                    mx = fmaxf(mx, __uint_as_float(lds32(other_at)));
+                    if (mx > kUnset) m = ceilf(mx);   // (not where no key is seen yet, and not for NaN)
+                    pair_sync();   // (the words are written again where a score passes the reference)
+                }
                 // Probabilities of 32 scores at a time against the reference as it is, their maximum found beside them.  Where a score of the
                 // row passes the reference by more than the slack (a row's first keys, hardly ever later) the reference, an integer,
                 // moves up in both of the row's threads, what has been summed and this tile's earlier probabilities are divided by the power of
