@@ -16,6 +16,13 @@
 // instruction cuts at the sum's last bit.  Softmax in base 2; a column's reference moves only when a score passes it by 2^8, and P is
 // held 2^7 times, so that small probabilities stay normal numbers.
 // Results do not depend on where pages lie; how the work is cut, and with it the last bits, depends on the call's lengths.
+//
+// What bounds it: issuing.  A page takes a warp about 330 instructions, 96 of them on the logic pipe, which starts one every other
+// clock, and three CTAs of four warps per SM issue two of three clocks: sixteen BF16 sequences of up to 32,768 keys, 32 / 8 heads, 395 MB,
+// 100 us, 61 % of the copy bandwidth.  Short calls are a chain of memory's latencies: where the CTA's run begins, queries and page
+// numbers, pages, and the merge's; one sequence of 1,024 keys takes 14 us with its append.  Tried: a grid of (span, item) instead of the
+// list 142 us for the sixteen, four CTAs per SM with 48 bytes of spills 103; for up to 16 columns three CTAs instead of two, 290 bytes of
+// spills, 175 against 166 us (40 sequences of four rows, windows of 4,096 keys), and blocks of 8 columns 189.
 #include <math.h>
 
 #include <algorithm>
@@ -135,7 +142,7 @@ constexpr int kRing = 4;   // page records per warp: one read, three on their wa
 
 // NT: column tiles of 8.  PAIR: F32 queries.
 template <int HD, int NT, bool PAIR>
-__global__ void __launch_bounds__(kWarps * 32, HD <= 128 && NT == 1 ? (PAIR ? 3 : 4) : 2) kvq4_span_kernel(const KvQ4Attention a) {
+__global__ void __launch_bounds__(kWarps * 32, HD <= 128 && NT == 1 ? 3 : 2) kvq4_span_kernel(const KvQ4Attention a) {
     constexpr int NG = HD / 32, WORDS = NG < 4 ? NG : 4, SUB = NG / WORDS;
     constexpr int RECORD = q4_record(HD), RING = kRing, REC = HD + 2;
     constexpr int BLOCK = kQ4Page * 16 * WORDS;   // bytes of codes of one sub
@@ -599,7 +606,9 @@ bool aligned16(const void* p, long long stride, int size) { return (reinterpret_
 // Columns per CTA, and how many CTAs share the list.
 void plan_spans(KvQ4Attention& a) {
     const int group = a.q_heads / a.kv_heads;
-    a.tile_above = a.head_dim == 256 ? 0x7fffffff : 32;
+    // More columns take the tensor-memory kernel: eight BF16 sequences of 2,000 keys with 64 columns 55 us here and 80 there, with 128 91 and
+    // 66.  (Heads of 256 have no such kernel: two tiles' sums would fill tensor memory.)
+    a.tile_above = a.head_dim == 256 ? 0x7fffffff : 64;
     const int cols = (int)std::min<long long>((long long)std::min(a.max_rows, a.rows) * group, a.tile_above);
     // 16 columns share a page's conversion; with heads of 256 their sums do not fit in the registers (1,080 bytes of spills)
     a.span_cols = cols <= 8 || a.head_dim == 256 ? 8 : 16;
@@ -607,7 +616,7 @@ void plan_spans(KvQ4Attention& a) {
     a.merge_cols = std::min(cols, a.span_cols);
     const long long keys = a.window > 0 ? std::min<long long>(a.max_keys, (long long)a.window + a.max_rows + kQ4Page) : a.max_keys;
     const long long pages = std::max(1ll, (keys + kQ4Page - 1) / kQ4Page), items = (long long)a.sequences * a.kv_heads * a.col_blocks;
-    const long long resident = (long long)kvq4_sm_count() * (a.head_dim <= 128 && a.span_cols == 8 ? (a.type == kQ4F32 ? 3 : 4) : 2);
+    const long long resident = (long long)kvq4_sm_count() * (a.head_dim <= 128 && a.span_cols == 8 ? 3 : 2);   // as their launch bounds say
     a.least_pages = kWarps;
     a.grid = (int)std::max(1ll, std::min(resident, (items * pages + a.least_pages - 1) / a.least_pages));
     a.max_spans = 2;   // an item may be cut, unless one CTA has all
