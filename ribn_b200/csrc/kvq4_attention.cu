@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 && NT == 1 ? 3 : 2) kvq
     const long long share = share_of(a, total);
     long long at = blockIdx.x * share;
     const long long stop = min(total, at + share);
-    if (blockIdx.x == 0 && a.max_spans > 1) {   // for the merge
+    if (blockIdx.x == 0 && a.may_cut) {   // for the merge
         long long x = before;
         for (int i = s0; i < s1; ++i) { a.prefix[i] = x; x += sequence_of(a, i).weight(a.kv_heads); }
         if (threadIdx.x == 0) a.prefix[a.sequences] = total;
@@ -619,8 +619,7 @@ void plan_spans(KvQ4Attention& a) {
     const long long resident = (long long)kvq4_sm_count() * (a.head_dim <= 128 && a.span_cols == 8 ? 3 : 2);   // as their launch bounds say
     a.least_pages = kWarps;
     a.grid = (int)std::max(1ll, std::min(resident, (items * pages + a.least_pages - 1) / a.least_pages));
-    a.max_spans = 2;   // an item may be cut, unless one CTA has all
-    if (a.grid == 1) a.max_spans = 1;
+    a.may_cut = a.grid > 1;   // an item may have runs in several CTAs
 }
 
 template <typename Kernel>
@@ -661,7 +660,7 @@ cudaError_t launch_hd(cudaStream_t stream, const KvQ4Attention& a) {
     const bool pair = a.type == kQ4F32;
     cudaError_t e = a.span_cols == 8 ? (pair ? launch_spans<HD, 1, true>(stream, a) : launch_spans<HD, 1, false>(stream, a))
                                      : (pair ? launch_spans<HD, WIDE, true>(stream, a) : launch_spans<HD, WIDE, false>(stream, a));
-    if (e == cudaSuccess && a.max_spans > 1) e = launch(stream, kvq4_merge_kernel<HD>, (long long)a.sequences * a.kv_heads * a.col_blocks * a.merge_cols, 0, a);
+    if (e == cudaSuccess && a.may_cut) e = launch(stream, kvq4_merge_kernel<HD>, (long long)a.sequences * a.kv_heads * a.col_blocks * a.merge_cols, 0, a);
     return e;
 }
 
@@ -682,7 +681,7 @@ namespace {
 constexpr size_t kScratchMost = 512u << 20;
 size_t prefix_bytes(const KvQ4Attention& a) { return ((size_t)a.sequences + 1) * sizeof(long long); }
 size_t partial_bytes(const KvQ4Attention& a) {
-    const size_t n = a.max_spans > 1 ? prefix_bytes(a) + (size_t)a.grid * 2 * a.span_cols * (a.head_dim + 2) * sizeof(float) : 0;
+    const size_t n = a.may_cut ? prefix_bytes(a) + (size_t)a.grid * 2 * a.span_cols * (a.head_dim + 2) * sizeof(float) : 0;
     return (n + 255) / 256 * 256;
 }
 bool has_tiles(const KvQ4Attention& a) { return (long long)std::min(a.max_rows, a.rows) * (a.q_heads / a.kv_heads) > a.tile_above; }

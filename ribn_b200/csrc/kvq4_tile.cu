@@ -41,6 +41,8 @@ constexpr uint32_t kSpinLimit = 1u << 22;
 constexpr float kLog2e = 1.4426950408889634f, kHeld = 7.0f, kSlack = 8.0f;
 constexpr int kPolynomial = 4;   // of 16 pairs of probabilities: those whose exponentials the multiply-add pipe computes
 constexpr float kUnset = -3e38f;   // below every finite score's place
+// PAIR: shares of the 512 x 128 registers at launch, 256 x (192 + 64).  (The other form keeps its 768 x 80.)
+constexpr int kSoftmaxRegs = 192, kOtherRegs = 64;
 constexpr int kWindow = 2;   // PAIR: key tiles whose products one sum in tensor memory holds
 
 template <int HD, bool PAIR>
@@ -56,8 +58,6 @@ struct Tile {
     // threads that share a query row's keys
     static constexpr int HALVES = PAIR ? 1 : 2;
     static constexpr int K_WARP = 8 * HALVES, MMA_WARP = K_WARP + kKWarps, V_WARP = MMA_WARP + 1, THREADS = (V_WARP + kVWarps) * 32;
-    // 512 x 128 registers at launch of F32 rows' form: 256 x (192 + 64).  The other keeps its 768 x 80.
-    static constexpr int SOFTMAX_REGS = 192, OTHER_REGS = 64;
 };
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
@@ -79,13 +79,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
                  "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
                  "r"(r[14]), "r"(r[15]) : "memory");
-}
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
-        "%30,%31,%32};" ::"r"(taddr), "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]), "f"(r[8]), "f"(r[9]), "f"(r[10]), "f"(r[11]),
-        "f"(r[12]), "f"(r[13]), "f"(r[14]), "f"(r[15]), "f"(r[16]), "f"(r[17]), "f"(r[18]), "f"(r[19]), "f"(r[20]), "f"(r[21]), "f"(r[22]), "f"(r[23]), "f"(r[24]),
-        "f"(r[25]), "f"(r[26]), "f"(r[27]), "f"(r[28]), "f"(r[29]), "f"(r[30]), "f"(r[31]) : "memory");
 }
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
@@ -157,7 +150,7 @@ __device__ __forceinline__ constexpr int key_of_place(int p) { return 2 * (p >> 
 
 // Where a sequence's key tiles lie among those of all sequences of this kernel: [first, first + count) from key tile `tile0` on.
 struct Tiles {
-    int first, count, tile0, low, high;   // keys low <= key < high are seen by some row
+    int first, count, tile0;
 };
 __device__ __forceinline__ int tiles_of(const KvQ4Attention& a, int s, int& tile0, int& low, int& high) {
     const int group = a.q_heads / a.kv_heads, begin = a.cu_rows[s], end = a.cu_rows[s + 1], length = a.lengths[s];
@@ -178,7 +171,8 @@ __device__ __forceinline__ Tiles tiles_before(const KvQ4Attention& a, int s, int
     }
     Tiles r;
     r.first = __reduce_add_sync(0xffffffffu, before);
-    r.count = tiles_of(a, s, r.tile0, r.low, r.high);
+    int low, high;   // keys that some row sees
+    r.count = tiles_of(a, s, r.tile0, low, high);
     return r;
 }
 
@@ -283,7 +277,7 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
     bool alive = true;
 
     if (warp >= T::K_WARP) {
-        if constexpr (PAIR) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::OTHER_REGS));
+        if constexpr (PAIR) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         if (warp == T::MMA_WARP) {
             // ---------------- products (the warp as a whole, one elected lane in it) ----------------
             // (trip counts that the compiler knows to be the warp's keep addresses and descriptors in uniform registers)
@@ -506,7 +500,7 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
         }
     } else {
         // ---------------- softmax: one row per thread ----------------
-        if constexpr (PAIR) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T::SOFTMAX_REGS));
+        if constexpr (PAIR) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         constexpr int HALVES = T::HALVES, DH = HD / HALVES;   // dimensions of the result that a thread has
         const int t = warp / (4 * HALVES), part = (warp >> 2) % HALVES, row0 = (warp & 3) * 32, row = row0 + lane, flat0 = w.flat0 + t * kRows;
         const uint32_t q_tile = at + T::PLANES * t * T::Q_TILE;
