@@ -114,8 +114,8 @@ def attention(cache: torch.Tensor, q: torch.Tensor, page_tables: torch.Tensor, l
     sequences, width = page_tables.shape
     tables, at_lengths = _ints("page_tables", page_tables, (sequences, width), device), _ints("lengths", lengths, (sequences,), device)
     at_rows = _ints("cu_rows", cu_rows, (sequences + 1,), device)
-    if scale is not None and not 0.0 < abs(scale) < float("inf"):
-        raise ValueError("scale must be finite and not zero")
+    if scale is not None and not 1.2e-38 <= abs(scale) <= 3.4e38:   # zero would stand for the default
+        raise ValueError("scale must be a float32 number other than zero")
     if out is None:
         out = torch.zeros((rows, q_heads, head_dim), dtype=q.dtype, device=q.device)
     out_stride = _rows("out", out, q_heads, head_dim, device, rows, q.dtype)

@@ -466,7 +466,7 @@ def test_refusals_of_the_python_calls(kvq4):
     good = dict(max_rows=1, max_keys=32)
     for args, more in (((q[:, :3], tables, lengths, cu), good), ((q, tables[:2], lengths, cu), good), ((q, tables, lengths, cu[:3]), good),
                        ((q, tables.long(), lengths, cu), good), ((q, tables.t(), lengths, cu), good), ((q, tables, lengths, cu), dict(good, scale=0.0)),
-                       ((q, tables, lengths, cu), dict(good, scale=float("nan"))), ((q, tables, lengths, cu), dict(good, out=q.float())),
+                       ((q, tables, lengths, cu), dict(good, scale=float("nan"))), ((q, tables, lengths, cu), dict(good, scale=1e-50)), ((q, tables, lengths, cu), dict(good, scale=-1e39)), ((q, tables, lengths, cu), dict(good, out=q.float())),
                        ((q, tables, lengths, cu), dict(good, out=q[:2]))):
         with pytest.raises(ValueError):
             kvq4.attention(cache, *args, **more)
