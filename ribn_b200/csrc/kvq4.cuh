@@ -56,7 +56,7 @@ struct KvQ4Attention {
     float* partial;                    // scratch of partial_bytes: the runs' sums and the operands below
     size_t partial_bytes;
     // set by the launcher
-    int grid, least_pages, may_cut, span_cols, col_blocks, merge_cols, vector_q, vector_out;
+    int grid, least_pages, set_up, may_cut, span_cols, col_blocks, merge_cols, vector_q, vector_out;
     long long* prefix;                 // pages of the span kernel's list before each sequence, and of all
     unsigned char* scratch;            // operands of the tile kernel's key tiles, [tile][kv_head][512 head_dim bytes]
     int scratch_tiles;                 // how many tiles there is room for

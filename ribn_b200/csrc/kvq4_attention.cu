@@ -90,17 +90,14 @@ __device__ __forceinline__ void store_value(const KvQ4Attention& a, long long at
     else asm volatile("{\n\t.reg .b16 t;\n\tcvt.rn.bf16.f32 t, %1;\n\tst.global.b16 [%0], t;\n\t}" ::"l"(static_cast<unsigned short*>(a.out) + at), "f"(x) : "memory");
 }
 
-constexpr int kSetUp = 40;
-
 // A sequence in the list of work.  Its row i is at position base + i.
 struct Sequence {
     int row0, n, base;
     int page0, pages;      // that some row sees
     int blocks;            // of columns
-    // Of an item, in pages: its set-up and fold, a chain of memory's latencies, take as long as kSetUp of them.  (Counted as 8, CTAs with
-    // many short items were the last ones by far: 40 sequences of four rows behind windows of 4,096 keys, a tenth of them with four
-    // keys, 264 us; as 24, 213; as 40, 172.)  One without keys writes its zeros.
-    __device__ __forceinline__ int length() const { return pages > 0 ? pages + kSetUp : 1; }
+    int set_up;            // see plan_spans
+    // of an item, in pages; one without keys writes its zeros
+    __device__ __forceinline__ int length() const { return pages > 0 ? pages + set_up : 1; }
     __device__ __forceinline__ long long weight(int kv_heads) const { return (long long)kv_heads * blocks * length(); }
 };
 __device__ __forceinline__ Sequence sequence_of(const KvQ4Attention& a, int s) {
@@ -111,6 +108,7 @@ __device__ __forceinline__ Sequence sequence_of(const KvQ4Attention& a, int s) {
     q.base = min(max(a.lengths[s], 0), a.pages_per_sequence * kQ4Page) - q.n;
     const int high = max(0, q.base + q.n), low = a.window > 0 ? max(0, q.base - a.window + 1) : 0;
     q.page0 = low / kQ4Page;
+    q.set_up = a.set_up;
     q.pages = high > low ? (high + kQ4Page - 1) / kQ4Page - q.page0 : 0;
     const long long cols = (long long)min(q.n, a.max_rows) * group;
     q.blocks = cols > a.tile_above ? 0 : (int)((cols + a.span_cols - 1) / a.span_cols);   // 0: the tile kernel's
@@ -207,8 +205,8 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 && NT == 1 ? 3 : 2) kvq
     const bool whole = run == seq.length();
     const Block b = block_of(a, seq, cb);
     // the run's pages, those that the block sees
-    const int begin = max(seq.page0 + max(offset - kSetUp, 0), b.low / kQ4Page);
-    const int end = max(begin, min(seq.page0 + max(min(offset + run - kSetUp, seq.pages), 0), (b.high + kQ4Page - 1) / kQ4Page));
+    const int begin = max(seq.page0 + max(offset - seq.set_up, 0), b.low / kQ4Page);
+    const int end = max(begin, min(seq.page0 + max(min(offset + run - seq.set_up, seq.pages), 0), (b.high + kQ4Page - 1) / kQ4Page));
     at += run;
     if (begin == end) {   // none: zeros, or a share of the item that counts for nothing
         for (int i = threadIdx.x; i < b.cols * REC; i += kWarps * 32) {
@@ -614,6 +612,11 @@ void plan_spans(KvQ4Attention& a) {
     a.span_cols = cols <= 8 || a.head_dim == 256 ? 8 : 16;
     a.col_blocks = (cols + a.span_cols - 1) / a.span_cols;
     a.merge_cols = std::min(cols, a.span_cols);
+    // An item's set-up and fold, a chain of memory's latencies, count as this many pages.  (As 8, CTAs with many short items were the last
+    // ones by far.)  16 columns, 40 sequences of four rows behind windows of 4,096 keys, a tenth of them with four keys: as 20 220 us, 40
+    // 165, 64 159, but 64 even sequences of 4,096 keys as 40 138 and as 64 142.  8 columns, 64 sequences of up to 1,500 keys: as 20 45.9,
+    // 40 47.0, 64 47.4; sixteen of up to 32,768: 98.6, 100.5, 102.5.
+    a.set_up = a.span_cols == 8 ? 20 : 40;
     const long long keys = a.window > 0 ? std::min<long long>(a.max_keys, (long long)a.window + a.max_rows + kQ4Page) : a.max_keys;
     const long long pages = std::max(1ll, (keys + kQ4Page - 1) / kQ4Page), items = (long long)a.sequences * a.kv_heads * a.col_blocks;
     const long long resident = (long long)kvq4_sm_count() * (a.head_dim <= 128 && a.span_cols == 8 ? 3 : 2);   // as their launch bounds say
