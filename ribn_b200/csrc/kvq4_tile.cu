@@ -734,6 +734,7 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
                             hi[u] = as_bits(__floats2half2_rn(p.x, p.y));
                         }
                         if (!pair_any(mx > m + kSlack)) break;
+                        tmem_wait_st();   // what is read back below may have been stored in this tile: earlier probabilities, sums of an earlier move
                         asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine_at), "f"(mx) : "memory");
                         pair_sync();
                         mx = fmaxf(mx, __uint_as_float(lds32(other_at)));

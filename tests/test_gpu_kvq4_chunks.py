@@ -1,0 +1,71 @@
+"""Attention of many rows over the 4-bit KV cache (ribn_b200.kvq4), where its kernel for them has several key tiles of 128 in one CTA, moves
+its references late, or meets what no row may see.  Against the 64-bit reference (tests/kvq4_reference.py), whose keys and values are what the
+arena stands for (read back as F32, which is exact); tolerances are those of tests/test_gpu_kvq4.py.
+
+A sequence with more than 64 query rows per kv head takes that kernel (`_MANY`).  `max_keys`, a hint, chooses its form: as 1 a CTA has all of a pair
+of query tiles' keys and converts the pages itself, with the true length the keys are shared among CTAs while they leave SMs idle, and
+come expanded from the scratch; 75 kv heads leave no SM idle."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+from tests import kvq4_reference as R  # noqa: E402
+from tests.test_gpu_kvq4 import TYPES, _check, _host, _rows, _tables  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+_MANY = 65   # query rows per kv head
+
+
+@pytest.fixture(scope="module")
+def kvq4(built_library):
+    from ribn_b200 import kvq4 as module
+    return module
+
+
+class _Cache:
+    """An arena with rows k, v at its first slots, and the values that it stands for."""
+
+    def __init__(self, kvq4, k, v, pages=None):
+        rows, heads, d = k.shape
+        self.pages = pages or (rows + 15) // 16
+        self.bytes = kvq4.empty_cache(self.pages, heads, d)
+        slots = torch.arange(self.pages * 16, dtype=torch.int32, device="cuda")
+        kvq4.append(self.bytes, k, v, slots[:rows])
+        self.k, self.v = (_host(x) for x in kvq4.read(self.bytes, slots, dtype=torch.float32))
+
+
+def _attend(kvq4, cache, q, tables, lengths, cu, max_keys=None, window=0, scale=None, unit=0.0, check=True):
+    cut = [b - a for a, b in zip(cu, cu[1:])]
+    got = kvq4.attention(cache.bytes, q, torch.from_numpy(tables).cuda(), torch.tensor(lengths, dtype=torch.int32, device="cuda"),
+                         torch.tensor(cu, dtype=torch.int32, device="cuda"), max_rows=max(cut), max_keys=max(lengths) if max_keys is None else max_keys,
+                         window=window, scale=scale)
+    if check:
+        with np.errstate(invalid="ignore"):
+            want, sizes = R.attention(cache.k, cache.v, cache.pages, _host(q), tables, lengths, cu, window, q.shape[2] ** -0.5 if scale is None else scale, np.zeros(q.shape))
+        _check(got, want, sizes, q.dtype, unit)
+    return got
+
+
+@pytest.mark.parametrize("type_name", TYPES)
+@pytest.mark.parametrize("heads,hint", [(1, 1), (1, 1000), (75, 1000)])
+@pytest.mark.parametrize("step", [7.0, -7.0])
+def test_scores_that_rise_from_keys_to_keys(kvq4, type_name, heads, hint, step):
+    """Scores grow by 2^10 from every 32 keys to the next 32, so that a row's reference moves in both halves of a key tile, tile after tile, and what
+    has been summed (results in tensor memory, this tile's earlier probabilities) is scaled again and again; rows of other signs and sizes beside them."""
+    dtype, unit = TYPES[type_name]
+    rng = np.random.default_rng(21)
+    keys, d = 1000, 64
+    k = rng.normal(0, 0.05, (keys, heads, d)).astype(np.float32)
+    k[:, :, 5] = step * (np.arange(keys) // 32)[:, None]
+    cache = _Cache(kvq4, torch.from_numpy(k).cuda(), _rows(rng, keys, heads, d, torch.float32))
+    q = rng.normal(0, 1, (_MANY, heads, d)).astype(np.float32)
+    q[:, :, 5] = rng.choice([4.0, 4.0, 4.0, 8.0, -4.0, 0.0, 1.0], (_MANY, heads))
+    tables = rng.permutation(cache.pages).astype(np.int32)[None]
+    # (pages anywhere, the scores by position: the reference's arrays lie by slot, as the arena does)
+    order = torch.empty_like(cache.bytes)
+    order[torch.from_numpy(tables[0]).long().cuda()] = cache.bytes
+    at = (tables[0][:, None] * 16 + np.arange(16)).reshape(-1)
+    cache.bytes = order
+    cache.k, cache.v = (np.stack([x[i] for i in np.argsort(at)]) for x in (cache.k, cache.v))
+    _attend(kvq4, cache, torch.from_numpy(q).to(dtype).cuda(), tables, [keys], [0, _MANY], max_keys=hint, scale=0.25, unit=unit)
