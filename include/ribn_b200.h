@@ -487,7 +487,8 @@ RIBN_B200_API int ribn_b200_kvq4_read(int32_t device, void* stream, const void* 
  * 1 / sqrt(head_dim).  `q_stride`, `out_stride`: values from one row to the next; `out` does not overlap `q`.  At most 2^26 pages
  * per sequence.  `workspace` (16-byte aligned, what ribn_b200_kvq4_workspace asks for; the part that it asks for operands of
  * sequences with many rows may be missing, which is slower) is scratch of this call: calls that may overlap on the GPU, or graphs that may replay
- * at once, need one each. */
+ * at once, need one each.  The kernel of sequences with many rows waits for its own warps with a limit of 2^22 polls; should one run out, the
+ * call still ends, and the rows concerned are NaN. */
 typedef struct {
     const void* cache;
     int64_t pages;
@@ -506,6 +507,8 @@ typedef struct {
 } ribn_b200_kvq4_attention_args;
 RIBN_B200_API size_t ribn_b200_kvq4_workspace(const ribn_b200_kvq4_attention_args* args);
 RIBN_B200_API int ribn_b200_kvq4_attention(int32_t device, void* stream, const ribn_b200_kvq4_attention_args* args);
+/* Test aid: the same call with barrier waits (of sequences with many rows) that run out after `wait_polls` polls, 0: at once. */
+RIBN_B200_API int ribn_b200_debug_kvq4_attention(int32_t device, void* stream, const ribn_b200_kvq4_attention_args* args, uint32_t wait_polls);
 
 /* Host-side tile-major repack used by finalize (no device work): writes the
  * packed form of raw GGUF rows and returns its size; `out` may be NULL to

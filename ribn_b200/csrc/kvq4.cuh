@@ -22,6 +22,7 @@ namespace ribn {
 
 constexpr int kQ4Page = 16;            // tokens per page
 constexpr int kQ4MaxGroup = 16;        // query heads per kv head
+constexpr uint32_t kQ4WaitPolls = 1u << 22;
 __host__ __device__ constexpr int q4_record(int head_dim) { return 18 * head_dim; }
 
 enum Q4Type : int { kQ4F32 = 0, kQ4F16 = 1, kQ4BF16 = 2 };
@@ -53,6 +54,7 @@ struct KvQ4Attention {
     const int32_t* cu_rows;            // [sequences + 1]
     int sequences, rows, max_rows, max_keys, window;
     float scale;                       // of the scores
+    uint32_t wait_polls;               // of a barrier in the tile kernel, before the wait has run out
     float* partial;                    // scratch of partial_bytes: the runs' sums and the operands below
     size_t partial_bytes;
     // set by the launcher

@@ -72,6 +72,30 @@ const char* bad_attention(const ribn_b200_kvq4_attention_args& a) {
     return nullptr;
 }
 
+int attend(int32_t device, void* stream, const ribn_b200_kvq4_attention_args* args, uint32_t wait_polls) {
+    if (args == nullptr) return op_error("kvq4_attention: null argument", cudaSuccess);
+    const ribn_b200_kvq4_attention_args& x = *args;
+    if (const char* why = bad_arena(x.cache, x.pages, x.kv_heads, x.head_dim, x.type)) return op_error(why, cudaSuccess);
+    if (const char* why = bad_attention(x)) return op_error(why, cudaSuccess);
+    if (!(fabsf(x.scale) < INFINITY)) return op_error("kvq4_attention: scale must be finite", cudaSuccess);
+    if (x.rows == 0 || x.sequences == 0 || x.max_rows == 0) return RIBN_B200_OK;
+    if (x.q == nullptr || x.out == nullptr || x.lengths == nullptr || x.cu_rows == nullptr || (x.page_tables == nullptr && x.pages_per_sequence > 0)) {
+        return op_error("kvq4_attention: null device pointer", cudaSuccess);
+    }
+    if (misaligned(x.q, x.type) || misaligned(x.out, x.type)) return op_error("kvq4_attention: q or out is not aligned to its type", cudaSuccess);
+    const int64_t width = (int64_t)x.q_heads * x.head_dim;
+    if ((x.rows > 1 && (x.q_stride < width || x.out_stride < width)) || x.q_stride < 0 || x.out_stride < 0 ||
+        (x.sequences > 1 && x.table_stride < x.pages_per_sequence) || x.table_stride < 0) {
+        return op_error("kvq4_attention: a stride below the length of its rows", cudaSuccess);
+    }
+    if ((reinterpret_cast<uintptr_t>(x.workspace) & 15) != 0) return op_error("kvq4_attention: the workspace must be 16-byte aligned", cudaSuccess);
+    return on_device(device, "kvq4_attention", [&]() -> cudaError_t {
+        KvQ4Attention a = attention_of(x);
+        a.wait_polls = wait_polls;
+        return launch_kvq4_attention(static_cast<cudaStream_t>(stream), a);
+    });
+}
+
 }  // namespace
 
 extern "C" {
@@ -109,26 +133,11 @@ size_t ribn_b200_kvq4_workspace(const ribn_b200_kvq4_attention_args* args) {
 }
 
 int ribn_b200_kvq4_attention(int32_t device, void* stream, const ribn_b200_kvq4_attention_args* args) {
-    if (args == nullptr) return op_error("kvq4_attention: null argument", cudaSuccess);
-    const ribn_b200_kvq4_attention_args& x = *args;
-    if (const char* why = bad_arena(x.cache, x.pages, x.kv_heads, x.head_dim, x.type)) return op_error(why, cudaSuccess);
-    if (const char* why = bad_attention(x)) return op_error(why, cudaSuccess);
-    if (!(fabsf(x.scale) < INFINITY)) return op_error("kvq4_attention: scale must be finite", cudaSuccess);
-    if (x.rows == 0 || x.sequences == 0 || x.max_rows == 0) return RIBN_B200_OK;
-    if (x.q == nullptr || x.out == nullptr || x.lengths == nullptr || x.cu_rows == nullptr || (x.page_tables == nullptr && x.pages_per_sequence > 0)) {
-        return op_error("kvq4_attention: null device pointer", cudaSuccess);
-    }
-    if (misaligned(x.q, x.type) || misaligned(x.out, x.type)) return op_error("kvq4_attention: q or out is not aligned to its type", cudaSuccess);
-    const int64_t width = (int64_t)x.q_heads * x.head_dim;
-    if ((x.rows > 1 && (x.q_stride < width || x.out_stride < width)) || x.q_stride < 0 || x.out_stride < 0 ||
-        (x.sequences > 1 && x.table_stride < x.pages_per_sequence) || x.table_stride < 0) {
-        return op_error("kvq4_attention: a stride below the length of its rows", cudaSuccess);
-    }
-    if ((reinterpret_cast<uintptr_t>(x.workspace) & 15) != 0) return op_error("kvq4_attention: the workspace must be 16-byte aligned", cudaSuccess);
-    return on_device(device, "kvq4_attention", [&]() -> cudaError_t {
-        const KvQ4Attention a = attention_of(x);
-        return launch_kvq4_attention(static_cast<cudaStream_t>(stream), a);
-    });
+    return attend(device, stream, args, kQ4WaitPolls);
+}
+
+int ribn_b200_debug_kvq4_attention(int32_t device, void* stream, const ribn_b200_kvq4_attention_args* args, uint32_t wait_polls) {
+    return attend(device, stream, args, wait_polls < kQ4WaitPolls ? wait_polls : kQ4WaitPolls);
 }
 
 }  // extern "C"

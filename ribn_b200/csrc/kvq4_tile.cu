@@ -14,7 +14,7 @@
 // F32 queries and probabilities are binary16 hi + lo pairs, two products each, and a row has one thread; as an addition in tensor
 // memory cuts at the sum's last bit, their sums over 256 keys move into the rows' registers.
 // Roles of the 24 warps (16 of F32 rows): softmax and output of tile 0 and 1, four K, one issues the products, three V.  Every wait is
-// bounded; where one runs out the CTA's rows become NaN.
+// bounded; where one runs out the CTA's rows become NaN, and what it has in flight is waited for (with a limit too) before it ends.
 //
 // What bounds it: a tile's chain.  Its products take 1,024 clocks, its scores 1,300 to 1,600 to become probabilities (exponentials: 16 a
 // clock per SM, a quarter of them moved to the multiply-add pipe), and handing over costs about 700 each time, while the other tile's
@@ -37,7 +37,7 @@ namespace {
 
 constexpr int kRows = 128, kKeys = 128, kKWarps = 4, kVWarps = 3;
 constexpr int kTilePages = kKeys / kQ4Page;
-constexpr uint32_t kSpinLimit = 1u << 22;
+constexpr uint32_t kLandPolls = 1u << 14;   // a poll that fails takes 4 us: 65 ms for a copy to land
 constexpr float kLog2e = 1.4426950408889634f, kHeld = 7.0f, kSlack = 8.0f;
 constexpr int kPolynomial = 4;   // of 16 pairs of probabilities: those whose exponentials the multiply-add pipe computes
 constexpr float kUnset = -3e38f;   // below every finite score's place
@@ -274,7 +274,14 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
     const unsigned char* operands = a.scratch + ((long long)(tiles.first + first_tile - tiles.tile0) * a.kv_heads + kvh) * (T::K_TILE + T::V_TILE);
     const int32_t* table = a.page_tables + w.s * a.table_stride;
     const int table_pages = (high + kQ4Page - 1) / kQ4Page;   // those that some row looks at
+    // A wait that runs out says so to the whole CTA, whose rows become NaN: barriers may then be a phase apart, so that its others' are not to be trusted
     bool alive = true;
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+        if (alive) {
+            alive = mbar_wait(bar, parity & 1u, nullptr, 0, a.wait_polls);
+            if (!alive) asm volatile("st.shared.u32 [%0], %1;" ::"r"(failed), "r"(1) : "memory");
+        }
+    };
 
     if (warp >= T::K_WARP) {
         if constexpr (PAIR) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
@@ -284,9 +291,6 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
             const int n0 = __shfl_sync(0xffffffffu, n[0], 0), n1 = __shfl_sync(0xffffffffu, n[1], 0), n_all = max(n0, n1);
             const bool leader = elect_one();
             const uint32_t q_desc = umma_desc(at, T::Q_STRIDE), k_desc = umma_desc(at + T::K_AT, T::K_STRIDE), v_desc = umma_desc(at + T::V_AT, T::V_STRIDE);
-            auto wait = [&](uint32_t bar, uint32_t parity) {
-                if (alive) alive = mbar_wait(bar, parity & 1u, nullptr, 0, kSpinLimit);
-            };
             auto scores = [&](int t, int j) {
                 const uint32_t b = k_desc + (j % T::K_SLOTS) * (T::K_TILE >> 4), hi = q_desc + T::PLANES * t * (T::Q_TILE >> 4);
                 if (leader && alive) {
@@ -319,14 +323,12 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
                         umma_ts(o_at, p_at + 32 * (i >> 1) + 8 * (i & 1), b + i * (2 * T::V_STRIDE >> 4), umma_idesc(HD), PAIR ? 1u : goes_on | (uint32_t)(i != 0));
                     }
                 }
-                if (leader && j + 1 == count) {
-                    if (!alive) asm volatile("st.shared.u32 [%0], %1;" ::"r"(failed), "r"(1) : "memory");
-                    umma_commit(o_full + 8 * t);
-                }
+                if (leader && j + 1 == count) umma_commit(o_full + 8 * t);
             };
-            // (a slot that nobody asks for again is not given back: the arrival could come after the block's end)
-            auto release_k = [&](int j) { if (leader && j + T::K_SLOTS < n_all) umma_commit(k_empty + 8 * (j % T::K_SLOTS)); };
-            auto release_v = [&](int j) { if (leader && j + T::V_SLOTS < n_all) umma_commit(v_empty + 8 * (j % T::V_SLOTS)); };
+            // (a slot that nobody asks for again is not given back; nor is one after an expired wait, so that no loader fills a slot whose last
+            // filling may not be complete)
+            auto release_k = [&](int j) { if (leader && alive && j + T::K_SLOTS < n_all) umma_commit(k_empty + 8 * (j % T::K_SLOTS)); };
+            auto release_v = [&](int j) { if (leader && alive && j + T::V_SLOTS < n_all) umma_commit(v_empty + 8 * (j % T::V_SLOTS)); };
             // (a barrier costs a hundred clocks and more even where it is complete: K and V are waited for once a step, while the
             // probabilities are on their way anyhow)
             auto wait_k = [&](int j) { wait(k_full + 8 * (j % T::K_SLOTS), j / T::K_SLOTS); };
@@ -347,11 +349,9 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
                     if (t == 1 && j + 1 < n_all) release_k(j + 1);
                 }
             }
-            if (!alive) {
-                // let what was issued come to its end before the block, and its tensor memory, can
-                if (leader) umma_commit(drained);
-                mbar_wait(drained, 0, nullptr, 0, kSpinLimit);
-            }
+            // what was issued comes to its end before the block, and its tensor memory, can (the rows' threads may have given up)
+            if (leader) umma_commit(drained);
+            mbar_wait(drained, 0, nullptr, 0, kQ4WaitPolls);
         } else {
             // ---------------- page records to operands ----------------
             const unsigned char* head = a.cache + (long long)kvh * RECORD;
@@ -366,12 +366,6 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar);
             };
-            auto wait = [&](uint32_t bar, uint32_t parity) {
-                if (alive) {
-                    alive = mbar_wait(bar, parity & 1u, nullptr, 0, kSpinLimit);
-                    if (!alive && lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(failed), "r"(1) : "memory");
-                }
-            };
             const __half2 minus72 = __float2half2_rn(-72.0f);
             const bool is_k = warp < T::K_WARP + kKWarps;
             if (expanded) {   // a warp's share of each tile by one bulk copy
@@ -379,15 +373,20 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
                 const uint32_t full = is_k ? k_full : v_full, empty = is_k ? k_empty : v_empty, skip = is_k ? part * bytes : part * (T::V_TILE / 8 * 3), to = at + (is_k ? T::K_AT : T::V_AT) + skip;
                 const unsigned char* from = operands + (is_k ? 0 : T::K_TILE) + skip;
                 const long long step = (long long)a.kv_heads * (T::K_TILE + T::V_TILE);
-                for (int j = 0; j < n_tiles; ++j) {
+                int j = 0;
+                for (; j < n_tiles; ++j) {
                     const int slot = j % slots;
                     if (j >= slots) wait(empty + 8 * slot, j / slots - 1);
+                    if (__any_sync(0xffffffffu, !alive)) break;
                     if (lane == 0) {
                         mbar_expect_tx(full + 8 * slot, bytes);
                         bulk_g2s(to + slot * (is_k ? T::K_TILE : T::V_TILE), from + j * step, bytes, full + 8 * slot);
                     }
                     __syncwarp();
                 }
+                // the copies land before the block can end, whoever still waits for them (a phase that another loader has left incomplete is waited
+                // for to the limit)
+                for (int i = max(0, j - slots); i < j; ++i) mbar_wait(full + 8 * (i % slots), (uint32_t)(i / slots) & 1u, nullptr, 0, kLandPolls);
             } else if (is_k) {
                 int ids = look_up(0), next_ids = look_up(1);
                 // lane = (quarter t, row i of eight): eight lanes store 128 bytes side by side
@@ -410,6 +409,7 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
 #pragma unroll 1
                 for (int j = 0; j < n_tiles; ++j) {
                     if (j >= T::K_SLOTS) wait(k_empty + 8 * (j % T::K_SLOTS), j / T::K_SLOTS - 1);
+                    if (__any_sync(0xffffffffu, !alive)) break;
                     const uint32_t to = at + T::K_AT + (j % T::K_SLOTS) * T::K_TILE + t * T::K_STRIDE + place * 16;
 #pragma unroll 1
                     for (int page = kw; page < kTilePages; page += kKWarps) {
@@ -460,6 +460,7 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
 #pragma unroll 1
                 for (int j = 0; j < n_tiles; ++j) {
                     if (j >= T::V_SLOTS) wait(v_empty + 8 * (j % T::V_SLOTS), j / T::V_SLOTS - 1);
+                    if (__any_sync(0xffffffffu, !alive)) break;
                     const int key0 = (first_tile + j) * kKeys;
                     const bool edge = key0 < low || key0 + kKeys > high;   // what lies where no row looks may be anything
                     const uint32_t to = at + T::V_AT + (j % T::V_SLOTS) * T::V_TILE + (t >> 1) * T::V_STRIDE + g * 16 + (t & 1) * 8;
@@ -504,9 +505,6 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
         constexpr int HALVES = T::HALVES, DH = HD / HALVES;   // dimensions of the result that a thread has
         const int t = warp / (4 * HALVES), part = (warp >> 2) % HALVES, row0 = (warp & 3) * 32, row = row0 + lane, flat0 = w.flat0 + t * kRows;
         const uint32_t q_tile = at + T::PLANES * t * T::Q_TILE;
-        auto wait = [&](uint32_t bar, uint32_t parity) {
-            if (alive) alive = mbar_wait(bar, parity & 1u, nullptr, 0, kSpinLimit);
-        };
         // the two warps of a row block (not PAIR): a barrier of their own, which can also tell whether any of their threads says so
         const int pair_barrier = 1 + 4 * t + (warp & 3);
         auto pair_sync = [&]() { asm volatile("barrier.cta.sync.aligned %0, 64;" ::"r"(pair_barrier) : "memory"); };

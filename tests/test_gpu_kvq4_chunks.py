@@ -69,3 +69,39 @@ def test_scores_that_rise_from_keys_to_keys(kvq4, type_name, heads, hint, step):
     cache.bytes = order
     cache.k, cache.v = (np.stack([x[i] for i in np.argsort(at)]) for x in (cache.k, cache.v))
     _attend(kvq4, cache, torch.from_numpy(q).to(dtype).cuda(), tables, [keys], [0, _MANY], max_keys=hint, scale=0.25, unit=unit)
+
+
+@pytest.mark.parametrize("type_name", TYPES)
+@pytest.mark.parametrize("heads,d,hint", [(1, 128, 1), (1, 64, 900), (75, 64, 900)])
+def test_a_wait_that_runs_out_leaves_nan_and_nothing_else(kvq4, type_name, heads, d, hint):
+    """Waits of no or a few polls: the call ends, a row is as it should be or NaN as a whole, rows of the other kernel and the next call know nothing
+    of it.  Without a poll every row that sees a key is NaN."""
+    from ribn_b200 import lib
+    from ribn_b200._lib import KvQ4AttentionArgs
+    dtype, _ = TYPES[type_name]
+    rng = np.random.default_rng(22)
+    lengths, counts = [900, 300, 40], [_MANY, 1, 100]   # (the last one's first 60 rows see nothing)
+    cu = [0, *np.cumsum(counts).tolist()]
+    k, v = _rows(rng, 80 * 16, heads, d, dtype), _rows(rng, 80 * 16, heads, d, dtype)
+    cache, tables = kvq4.empty_cache(80, heads, d), _tables(rng, 80, lengths)
+    kvq4.append(cache, k, v, torch.arange(80 * 16, dtype=torch.int32, device="cuda"))
+    q = _rows(rng, cu[-1], heads, d, dtype)
+    keep = [torch.from_numpy(tables).cuda(), torch.tensor(lengths, dtype=torch.int32, device="cuda"), torch.tensor(cu, dtype=torch.int32, device="cuda")]
+    whole = kvq4.attention(cache, q, *keep, max_rows=100, max_keys=hint)
+    assert torch.isfinite(whole).all() and not whole[cu[2]:cu[2] + 60].any()
+    out = torch.empty_like(q)
+    args = KvQ4AttentionArgs(cache.data_ptr(), 80, q.data_ptr(), out.data_ptr(), keep[0].data_ptr(), keep[1].data_ptr(), keep[2].data_ptr(), None, 0,
+                             heads * d, heads * d, tables.shape[1], {"f32": 0, "f16": 1, "bf16": 2}[type_name], heads, heads, d, tables.shape[1], 3, cu[-1], 100, hint, 0, 0.0, 0)
+    scratch = torch.empty(lib().ribn_b200_kvq4_workspace(args), dtype=torch.uint8, device="cuda")
+    args.workspace, args.workspace_bytes = scratch.data_ptr(), scratch.numel()
+    for polls in (0, 1, 2, 3, 5, 8, 20, 1 << 30):
+        out.fill_(3.0)
+        assert lib().ribn_b200_debug_kvq4_attention(0, torch.cuda.current_stream().cuda_stream, args, polls) == 0
+        lost = torch.isnan(out).all(dim=2)
+        assert torch.equal(out[~lost], whole[~lost])
+        assert not lost[cu[1]].any()
+        if polls == 0:
+            assert lost[:_MANY].all() and lost[cu[2] + 60:].all()
+        if polls == 1 << 30:
+            assert not lost.any()
+        assert torch.equal(kvq4.attention(cache, q, *keep, max_rows=100, max_keys=hint), whole)
