@@ -91,7 +91,8 @@ __device__ __forceinline__ float exp2_approx(float x) {
 }
 // 2^x of a pair on the multiply-add pipe, whose instructions take two values each, beside the sixteen a clock of the special function
 // unit: x = n + f, n the nearest integer (left in the low bits of x + 3 x 2^22), 2^f by the polynomial of degree 3 that is nearest in
-// relative error over [-1/2, 1/2] (7.5e-5, found by Remez's exchange; binary16 is off by up to 4.9e-4), n added to the exponent.
+// relative error over [-1/2, 1/2] (7.5e-5, found by Remez's exchange; binary16 is off by up to 4.9e-4), n added to the exponent.  NaN does
+// not pass (it comes out as 2^-126): rows whose queries are not finite become NaN by their flag.
 __device__ __forceinline__ float2 exp2_pair(float2 x) {
     constexpr float kMagic = 12582912.0f;
     x = make_float2(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));
@@ -537,19 +538,24 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
 #pragma unroll 1
             for (int rg = GROUPS * part; rg < GROUPS * (part + 1); ++rg) {
                 const int r = row0 + rg * 8 + sub;
-                float x[PP][8], top = 0.0f;
+                float x[PP][8];
+                uint32_t top = 0;   // the largest magnitude's bits, which order as the values do, NaN above all
 #pragma unroll
                 for (int p = 0; p < PP; ++p) {
                     q4_values(next[p], a.type, x[p]);
 #pragma unroll
-                    for (int u = 0; u < 8; ++u) top = fmaxf(top, fabsf(x[p][u]));
+                    for (int u = 0; u < 8; ++u) top = max(top, __float_as_uint(x[p][u]) & 0x7fffffffu);
                 }
                 if (rg + 1 < GROUPS * (part + 1)) ask(rg + 1);
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                const int e = top > 0.0f && top < INFINITY ? max(-126, min(126, 140 - (int)(__float_as_uint(top) >> 23))) : 0;
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                // A row that is not finite is NaN where it sees a key.  Its operand is zero, so that its thread can tell, by the reference, whether it does;
+                // its factor's sign tells the thread.
+                const bool spoiled = top >= 0x7f800000u;
+                const uint32_t keep = spoiled ? 0u : 0xffffffffu;
+                const int e = top > 0 && !spoiled ? max(-126, min(126, 140 - (int)(top >> 23))) : 0;
                 const float up = __int_as_float((e + 127) << 23) * (a.scale < 0.0f ? -1.0f : 1.0f), f = __int_as_float((127 - e) << 23);
-                const float scaled = f * (fabsf(a.scale) * kLog2e);
+                const float scaled = (spoiled ? -f : f) * (fabsf(a.scale) * kLog2e);
                 if constexpr (HALVES == 1) {
                     const float of_row = __shfl_sync(0xffffffffu, scaled, lane & 7);
                     if ((lane >> 3) == rg) factor = of_row;
@@ -564,6 +570,8 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
                     for (int i = 0; i < 4; ++i) {
                         if (PAIR) split2(x[p][i] * up, x[p][i + 4] * up, h[i], l[i]);
                         else h[i] = as_bits(__floats2half2_rn(x[p][i] * up, x[p][i + 4] * up));
+                        h[i] &= keep;
+                        if (PAIR) l[i] &= keep;
                     }
                     const uint32_t to = q_tile + (p * 4 + pc) * T::Q_STRIDE + r * 16;
                     sts128(to, hi);
@@ -578,6 +586,8 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
                 factor = __uint_as_float(lds32(factors + row * 4));
             }
         }
+        const bool spoiled = factor < 0.0f;
+        factor = fabsf(factor);
         const bool have = row < live_rows;
         const int limit = have ? w.base + (flat0 + row) / group : -1, lowest = a.window > 0 ? limit - a.window + 1 : 0;
         // keys that every row of the warp sees
@@ -773,6 +783,8 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
         if (live_rows > row0) {
             constexpr int VALUE = PAIR ? 4 : 2, ROW_BYTES = DH * VALUE, PIECES = ROW_BYTES / 16, SWAP = PIECES < 8 ? PIECES - 1 : 7;
             float total = l.x + l.y;
+            const bool none = own == 0 || m == (PAIR ? -INFINITY : kUnset);   // no key seen
+            if (spoiled && !none) total = __int_as_float(0x7fffffff);
             if constexpr (HALVES == 2) {
                 asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine_at), "f"(total) : "memory");
                 pair_sync();
@@ -783,8 +795,7 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
             const bool shared = a.tile_splits > 1, have_row = row < live_rows;
             float* record = a.tile_partial + (((long long)(w.row0 + (flat0 + row) / group) * a.q_heads + kvh * group + (flat0 + row) % group) * a.tile_splits + split) * (HD + 4);
             if (shared && have_row && part == 0) {
-                const bool none = own == 0 || (!PAIR && m == kUnset) || (PAIR && m == -INFINITY);
-                record[HD] = !alive || lds32(failed) != 0 ? __int_as_float(0x7fffffff) : none && total == total ? -INFINITY : PAIR ? __fmul_rn(m, factor) : m;
+                record[HD] = !alive || lds32(failed) != 0 || total != total ? __int_as_float(0x7fffffff) : none ? -INFINITY : PAIR ? __fmul_rn(m, factor) : m;
                 record[HD + 1] = total;
             }
             const uint32_t stage = q_tile + ((warp & 3) * HALVES + part) * 32 * ROW_BYTES;

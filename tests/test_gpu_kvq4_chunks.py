@@ -105,3 +105,24 @@ def test_a_wait_that_runs_out_leaves_nan_and_nothing_else(kvq4, type_name, heads
         if polls == 1 << 30:
             assert not lost.any()
         assert torch.equal(kvq4.attention(cache, q, *keep, max_rows=100, max_keys=hint), whole)
+
+
+@pytest.mark.parametrize("type_name", TYPES)
+@pytest.mark.parametrize("rows,length", [(90, 90), (90, 400), (3, 3), (3, 400)])
+@pytest.mark.parametrize("window,hint", [(0, 1), (0, 4000), (1, 1), (1, 4000), (2, 1), (30, 4000)])
+def test_a_query_that_is_not_finite(kvq4, type_name, rows, length, window, hint):
+    """NaN and infinities in queries: NaN wherever the row sees a key, be it one or all, zeros where it sees none, and nothing in other rows."""
+    dtype, unit = TYPES[type_name]
+    rng = np.random.default_rng(23)
+    cache = _Cache(kvq4, _rows(rng, 450, 1, 64, torch.float32), _rows(rng, 450, 1, 64, torch.float32))
+    tables = np.arange(cache.pages, dtype=np.int32)[None]
+    tables[0, (length - rows) // 16 + 2] = -1   # in a window of one, sixteen rows see nothing
+    q = _rows(rng, rows, 2, 64, dtype)
+    for row, head, values in ((0, 0, [float("nan")]), (1, 1, [float("inf")]), (0, 1, [float("-inf")]), (2, 0, [float("inf"), float("-inf")]), (4, 0, [float("-inf")]),
+                              (17, 1, [float("nan"), float("inf")]), (34, 0, [float("nan")]), (35, 1, [float("inf")]), (65, 0, [float("inf")]), (89, 1, [float("nan")])):
+        if row < rows:
+            q[row, head, 10:10 + len(values)] = torch.tensor(values).to(dtype)
+    got = _attend(kvq4, cache, q, tables, [length], [0, rows], max_keys=hint, window=window, unit=unit)
+    assert torch.isnan(got[0, 0]).all() and torch.isnan(got[1, 1]).all() and torch.isfinite(got[0, 1]).logical_not().all()
+    if rows > 35 and window == 1 and (length - rows) % 16 == 0:
+        assert not got[34, 0].any() and not got[35, 1].any()
