@@ -121,4 +121,9 @@ __device__ __forceinline__ void q4_load8(const void* base, long long at, int typ
     q4_values(w, type, x);
 }
 
+// A row's score factor in base 2, of (2^-e of its queries) x |scale of the scores|, kept where every product with a sum of its scaled queries and
+// keys (at most 2^35: 256 x 2^14 x 2^13) is finite, and none with an infinity NaN.  Below 2^-126 all scores are as good as zero either way, above
+// 2^92 the largest one has all the weight either way (sums that differ do so by 2^-44 or more, the last bits' product).
+__device__ __forceinline__ float q4_factor(float x) { return fminf(fmaxf(x * 1.4426950408889634f, 1.17549435e-38f), 4.9517602e27f); }
+
 }  // namespace ribn

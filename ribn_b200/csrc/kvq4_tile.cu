@@ -38,7 +38,7 @@ namespace {
 constexpr int kRows = 128, kKeys = 128, kKWarps = 4, kVWarps = 3;
 constexpr int kTilePages = kKeys / kQ4Page;
 constexpr uint32_t kLandPolls = 1u << 14;   // a poll that fails takes 4 us: 65 ms for a copy to land
-constexpr float kLog2e = 1.4426950408889634f, kHeld = 7.0f, kSlack = 8.0f;
+constexpr float kHeld = 7.0f, kSlack = 8.0f;
 constexpr int kPolynomial = 4;   // of 16 pairs of probabilities: those whose exponentials the multiply-add pipe computes
 constexpr float kUnset = -3e38f;   // below every finite score's place
 // PAIR: shares of the 512 x 128 registers at launch, 256 x (192 + 64).  (The other form keeps its 768 x 80.)
@@ -555,7 +555,7 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
                 const uint32_t keep = spoiled ? 0u : 0xffffffffu;
                 const int e = top > 0 && !spoiled ? max(-126, min(126, 140 - (int)(top >> 23))) : 0;
                 const float up = __int_as_float((e + 127) << 23) * (a.scale < 0.0f ? -1.0f : 1.0f), f = __int_as_float((127 - e) << 23);
-                const float scaled = (spoiled ? -f : f) * (fabsf(a.scale) * kLog2e);
+                const float size = q4_factor(f * fabsf(a.scale)), scaled = spoiled ? -size : size;
                 if constexpr (HALVES == 1) {
                     const float of_row = __shfl_sync(0xffffffffu, scaled, lane & 7);
                     if ((lane >> 3) == rg) factor = of_row;

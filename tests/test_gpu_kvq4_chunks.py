@@ -126,3 +126,37 @@ def test_a_query_that_is_not_finite(kvq4, type_name, rows, length, window, hint)
     assert torch.isnan(got[0, 0]).all() and torch.isnan(got[1, 1]).all() and torch.isfinite(got[0, 1]).logical_not().all()
     if rows > 35 and window == 1 and (length - rows) % 16 == 0:
         assert not got[34, 0].any() and not got[35, 1].any()
+
+
+def _far_ends(kvq4, dtype, unit, rows, d):
+    """Scores so small that every key weighs the same, and so large that one key has all the weight, as queries and scale of the scores come near
+    the ends of F32's range (and of the queries' type); masked keys beside them."""
+    rng = np.random.default_rng(24)
+    length = rows + 130
+    cache = _Cache(kvq4, _rows(rng, length, 1, d, torch.float32), _rows(rng, length, 1, d, torch.float32))
+    tables = np.arange(cache.pages, dtype=np.int32)[None]
+    base = _rows(rng, rows, 2, d, torch.float32).clamp(-3, 3)
+    for size, scale in ((1e-30, 1e-12), (1e-30, -1.2e-38), (1e-7, 1.2e-38), (1e-4, -1e-36), (0.0, 1.2e-38)):
+        _attend(kvq4, cache, (base * size).to(dtype), tables, [length], [0, rows], scale=scale, unit=unit)
+    seen = np.arange(length)[None] <= np.arange(length - rows, length)[:, None]
+    for size, scale in ((1e38, 1.0), (1e38, -1e3), (1e38, 3.4e38), (2e4, 3.4e38), (1.0, -3.4e38), (1e-4, 3.4e38), (1e38, 1e-25)):
+        q = (base * size).to(dtype)
+        if not torch.isfinite(q).all():
+            continue   # (F16 ends at 65,504)
+        got = _host(_attend(kvq4, cache, q, tables, [length], [0, rows], scale=scale, check=False))
+        x = np.einsum("rhd,kd->rhk", _host(q), cache.k[:length, 0]) * scale
+        x = np.where(seen[:, None], x, -np.inf)
+        order = np.argsort(x, axis=2)
+        best, next_best = (np.take_along_axis(x, order[..., [i]], 2)[..., 0] for i in (-1, -2))
+        clear = (best - next_best) > 2.0 ** -18 * np.max(np.abs(np.where(seen[:, None], x, 0.0)), axis=2)   # F32 sums of 128 products tell them apart
+        assert clear.mean() > 0.9 and np.min((best - next_best)[clear]) > 100.0
+        # one key's probability over itself: a polynomial exponential is off by less than 2^-13.7 in the sum, while its binary16 in the product is rounded back
+        want = cache.v[:length, 0][order[..., -1]]
+        allowed = np.abs(want) * (unit * (1 + 2.0 ** -8) + (2.0 ** -13.6 if dtype is not torch.float32 else 2.0 ** -19))
+        assert np.all(np.abs(got - want)[clear] <= allowed[clear]), (size, scale)
+
+
+@pytest.mark.parametrize("type_name", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+def test_scores_of_a_chunk_at_the_ends_of_the_range(kvq4, type_name, d):
+    _far_ends(kvq4, *TYPES[type_name], _MANY, d)
