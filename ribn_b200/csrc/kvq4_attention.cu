@@ -34,7 +34,6 @@ namespace ribn {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kHeld = 7.0f;    // P is held 2^7 times ..
 constexpr float kSlack = 8.0f;   // .. and may grow to 2^15
 
@@ -277,7 +276,7 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 && NT == 1 ? 3 : 2) kvq
         // 2^e brings the largest to [2^13, 2^14)
         const int e = top > 0.0f && top < INFINITY ? max(-126, min(126, 140 - (int)(__float_as_uint(top) >> 23))) : 0;
         const float up = __int_as_float((e + 127) << 23), down = __int_as_float((127 - e) << 23);
-        const float f = down * (a.scale * kLog2e * (PAIR ? 1.0f : 16777216.0f));   // (codes are held 2^-24 times)
+        const float f = copysignf(q4_factor(down * fabsf(a.scale)), a.scale) * (PAIR ? 1.0f : 16777216.0f);   // (codes are held 2^-24 times)
         factor[nt][0] = __shfl_sync(0xffffffffu, f, 8 * t);
         factor[nt][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
 #pragma unroll

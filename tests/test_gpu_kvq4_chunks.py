@@ -160,3 +160,9 @@ def _far_ends(kvq4, dtype, unit, rows, d):
 @pytest.mark.parametrize("d", [64, 128])
 def test_scores_of_a_chunk_at_the_ends_of_the_range(kvq4, type_name, d):
     _far_ends(kvq4, *TYPES[type_name], _MANY, d)
+
+
+@pytest.mark.parametrize("type_name", TYPES)
+@pytest.mark.parametrize("rows,d", [(1, 128), (5, 64), (3, 256), (20, 128)])
+def test_scores_of_few_rows_at_the_ends_of_the_range(kvq4, type_name, rows, d):
+    _far_ends(kvq4, *TYPES[type_name], rows, d)
