@@ -88,6 +88,7 @@ int attend(int32_t device, void* stream, const ribn_b200_kvq4_attention_args* ar
         (x.sequences > 1 && x.table_stride < x.pages_per_sequence) || x.table_stride < 0) {
         return op_error("kvq4_attention: a stride below the length of its rows", cudaSuccess);
     }
+    if (x.workspace == nullptr && x.workspace_bytes > 0) return op_error("kvq4_attention: null workspace with a size", cudaSuccess);
     if ((reinterpret_cast<uintptr_t>(x.workspace) & 15) != 0) return op_error("kvq4_attention: the workspace must be 16-byte aligned", cudaSuccess);
     return on_device(device, "kvq4_attention", [&]() -> cudaError_t {
         KvQ4Attention a = attention_of(x);
