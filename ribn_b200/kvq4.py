@@ -60,6 +60,14 @@ def _ints(name: str, x: torch.Tensor, shape: tuple, device: int):
     return x.data_ptr()
 
 
+_MOST = 2 ** 31 - 1
+
+
+def _size(x: int, most: int) -> int:
+    """A size for the C call, whose fields have 32 bits: one over `most` says what `most` says; a negative one is refused there."""
+    return -1 if x < 0 else min(x, most)
+
+
 # the stream as a number, without a Stream object around it, which takes longer to make than a small call
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
@@ -121,7 +129,7 @@ def attention(cache: torch.Tensor, q: torch.Tensor, page_tables: torch.Tensor, l
     out_stride = _rows("out", out, q_heads, head_dim, device, rows, q.dtype)
     args = KvQ4AttentionArgs(cache.data_ptr(), pages, q.data_ptr(), out.data_ptr(), tables, at_lengths, at_rows, None, 0, q_stride, out_stride,
                              page_tables.stride(0), _TYPES[q.dtype], q_heads, kv_heads, head_dim, width, sequences, rows,
-                             min(max_rows, rows), max_keys, window, scale or 0.0, 0)
+                             _size(max_rows, rows), _size(max_keys, _MOST - PAGE_TOKENS), _size(window, _MOST), scale or 0.0, 0)
     library = lib()
     need = library.ribn_b200_kvq4_workspace(args)
     if need:
