@@ -111,7 +111,8 @@ def attention(cache: torch.Tensor, q: torch.Tensor, page_tables: torch.Tensor, l
 
     Rows that see no key get zeros, rows behind the last sequence stay as they are in `out` (zeros in a new one).  `max_rows` is
     the most rows of a sequence; `max_keys`, about the longest length, decides how the work is split and no result.
-    `scale` defaults to head_dim ** -0.5.  Returns `out`, of q's type."""
+    `scale` defaults to head_dim ** -0.5.  There is no backward pass: a `q` or `out` that requires a gradient is refused while gradients
+    are recorded.  Returns `out`, of q's type."""
     pages, kv_heads, head_dim, device = _arena(cache)
     if q.dim() != 3 or q.shape[1] == 0 or q.shape[1] % kv_heads:
         raise ValueError(f"q must be [rows][q_heads][{head_dim}], q_heads a multiple of the cache's {kv_heads}")
@@ -124,6 +125,8 @@ def attention(cache: torch.Tensor, q: torch.Tensor, page_tables: torch.Tensor, l
     at_rows = _ints("cu_rows", cu_rows, (sequences + 1,), device)
     if scale is not None and not 1.2e-38 <= abs(scale) <= 3.4e38:   # zero would stand for the default
         raise ValueError("scale must be a float32 number other than zero")
+    if (q.requires_grad or (out is not None and out.requires_grad)) and torch.is_grad_enabled():
+        raise ValueError("attention over a 4-bit cache has no backward pass: call it under torch.no_grad() or with detached tensors")
     if out is None:
         out = torch.zeros((rows, q_heads, head_dim), dtype=q.dtype, device=q.device)
     out_stride = _rows("out", out, q_heads, head_dim, device, rows, q.dtype)

@@ -50,3 +50,15 @@ def test_sizes_beyond_32_bits(kvq4, rows):
     for bad in (dict(window=-1), dict(window=-2 ** 32 + 5), dict(max_keys=-2 ** 32 + 5), dict(max_rows=-2 ** 32 + 1)):
         with pytest.raises(RuntimeError, match="negative"):
             call(**bad)
+
+
+def test_a_query_that_wants_a_gradient_is_refused(kvq4):
+    call = _Call(kvq4)
+    whole = call()
+    q = call.q.clone().requires_grad_()
+    for change in (dict(q=q), dict(q=q * 2), dict(out=torch.zeros_like(call.q).requires_grad_())):
+        with pytest.raises(ValueError, match="no backward"):
+            call(**change)
+    with torch.no_grad():
+        assert torch.equal(call(q=q), whole)
+    assert torch.equal(call(q=q.detach()), whole)
