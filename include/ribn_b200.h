@@ -505,9 +505,11 @@ typedef struct {
     float scale;
     int32_t reserved;
 } ribn_b200_kvq4_attention_args;
+/* Enough for the call on any of the machine's devices, whichever is current. */
 RIBN_B200_API size_t ribn_b200_kvq4_workspace(const ribn_b200_kvq4_attention_args* args);
 RIBN_B200_API int ribn_b200_kvq4_attention(int32_t device, void* stream, const ribn_b200_kvq4_attention_args* args);
-/* Test aid: the same call with barrier waits (of sequences with many rows) that run out after `wait_polls` polls, 0: at once. */
+/* Test aids: the scratch that the call uses on a device of `sms` multiprocessors; the call with barrier waits (of sequences with many rows) that run out after `wait_polls` polls, 0: at once. */
+RIBN_B200_API size_t ribn_b200_debug_kvq4_workspace(const ribn_b200_kvq4_attention_args* args, int32_t sms);
 RIBN_B200_API int ribn_b200_debug_kvq4_attention(int32_t device, void* stream, const ribn_b200_kvq4_attention_args* args, uint32_t wait_polls);
 
 /* Host-side tile-major repack used by finalize (no device work): writes the

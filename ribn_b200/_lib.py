@@ -129,6 +129,7 @@ SIGNATURES = {
     "ribn_b200_kvq4_read": (C.c_int, [C.c_int32, _P, _P, C.c_int64, C.c_int32, C.c_int32, C.c_int32, _P, C.c_int64, _P, _P]),
     "ribn_b200_kvq4_workspace": (C.c_size_t, [C.POINTER(KvQ4AttentionArgs)]),
     "ribn_b200_kvq4_attention": (C.c_int, [C.c_int32, _P, C.POINTER(KvQ4AttentionArgs)]),
+    "ribn_b200_debug_kvq4_workspace": (C.c_size_t, [C.POINTER(KvQ4AttentionArgs), C.c_int32]),
     "ribn_b200_debug_kvq4_attention": (C.c_int, [C.c_int32, _P, C.POINTER(KvQ4AttentionArgs), C.c_uint32]),
     "ribn_b200_debug_step_deal": (C.c_int, [C.c_int32, C.c_int64, C.c_int64, C.c_int32, _P, C.c_size_t, C.POINTER(C.c_size_t),
                                             C.POINTER(C.c_size_t), C.POINTER(C.c_size_t)]),

@@ -58,6 +58,7 @@ struct KvQ4Attention {
     float* partial;                    // scratch of partial_bytes: the runs' sums and the operands below
     size_t partial_bytes;
     // set by the launcher
+    int sms;                           // of the device
     int grid, least_pages, set_up, may_cut, span_cols, col_blocks, merge_cols, vector_q, vector_out;
     long long* prefix;                 // pages of the span kernel's list before each sequence, and of all
     unsigned char* scratch;            // operands of the tile kernel's key tiles, [tile][kv_head][512 head_dim bytes]
@@ -67,7 +68,9 @@ struct KvQ4Attention {
     int tile_above;                    // a sequence with more query rows (rows x heads of a group) than this takes the tile kernel
 };
 // Bytes of scratch that launch_kvq4_attention can use; it works with less than the tile kernel's part, not with less than the sums.
-size_t kvq4_workspace_bytes(const KvQ4Attention& a);
+// It does not shrink with `sms`, so that asked for kvq4_most_sms() it does on every device.
+size_t kvq4_workspace_bytes(const KvQ4Attention& a, int sms);
+int kvq4_most_sms();
 cudaError_t launch_kvq4_attention(cudaStream_t stream, KvQ4Attention a);
 
 // The sequences with more than `tile_above` query rows (kvq4_tile.cu; heads of 64 and 128).

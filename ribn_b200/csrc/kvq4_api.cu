@@ -130,11 +130,17 @@ int ribn_b200_kvq4_read(int32_t device, void* stream, const void* cache, int64_t
 
 size_t ribn_b200_kvq4_workspace(const ribn_b200_kvq4_attention_args* args) {
     if (args == nullptr || bad_attention(*args) != nullptr || args->rows == 0 || args->sequences == 0 || args->max_rows == 0) return 0;
-    return kvq4_workspace_bytes(attention_of(*args));
+    static const int most_sms = kvq4_most_sms();
+    return kvq4_workspace_bytes(attention_of(*args), most_sms);
 }
 
 int ribn_b200_kvq4_attention(int32_t device, void* stream, const ribn_b200_kvq4_attention_args* args) {
     return attend(device, stream, args, kQ4WaitPolls);
+}
+
+size_t ribn_b200_debug_kvq4_workspace(const ribn_b200_kvq4_attention_args* args, int32_t sms) {
+    if (args == nullptr || bad_attention(*args) != nullptr || args->rows == 0 || args->sequences == 0 || args->max_rows == 0 || sms < 1) return 0;
+    return kvq4_workspace_bytes(attention_of(*args), sms);
 }
 
 int ribn_b200_debug_kvq4_attention(int32_t device, void* stream, const ribn_b200_kvq4_attention_args* args, uint32_t wait_polls) {

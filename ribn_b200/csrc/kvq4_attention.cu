@@ -618,7 +618,7 @@ void plan_spans(KvQ4Attention& a) {
     a.set_up = a.span_cols == 8 ? 20 : 40;
     const long long keys = a.window > 0 ? std::min<long long>(a.max_keys, (long long)a.window + a.max_rows + kQ4Page) : a.max_keys;
     const long long pages = std::max(1ll, (keys + kQ4Page - 1) / kQ4Page), items = (long long)a.sequences * a.kv_heads * a.col_blocks;
-    const long long resident = (long long)kvq4_sm_count() * (a.head_dim <= 128 && a.span_cols == 8 ? 3 : 2);   // as their launch bounds say
+    const long long resident = (long long)a.sms * (a.head_dim <= 128 && a.span_cols == 8 ? 3 : 2);   // as their launch bounds say
     a.least_pages = kWarps;
     a.grid = (int)std::max(1ll, std::min(resident, (items * pages + a.least_pages - 1) / a.least_pages));
     a.may_cut = a.grid > 1;   // an item may have runs in several CTAs
@@ -699,7 +699,7 @@ int wanted_tiles(const KvQ4Attention& a) {
 int wanted_splits(const KvQ4Attention& a) {
     if (!has_tiles(a)) return 1;
     const long long ctas = std::max(1ll, kvq4_tile_places(a) * a.kv_heads), tiles = std::max(1ll, seen_keys(a) / 128 + 1);
-    return (int)std::max(1ll, std::min(kvq4_sm_count() / ctas, (tiles + 1) / 2));
+    return (int)std::max(1ll, std::min(a.sms / ctas, (tiles + 1) / 2));
 }
 size_t split_bytes(const KvQ4Attention& a) {
     const int splits = wanted_splits(a);
@@ -708,14 +708,26 @@ size_t split_bytes(const KvQ4Attention& a) {
 
 }  // namespace
 
-size_t kvq4_workspace_bytes(const KvQ4Attention& args) {
+int kvq4_most_sms() {
+    int count = 0, most = 0;
+    if (cudaGetDeviceCount(&count) != cudaSuccess) count = 0;
+    for (int dev = 0; dev < count; ++dev) {
+        int sms = 0;
+        if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) most = std::max(most, sms);
+    }
+    return most > 0 ? most : 148;
+}
+
+size_t kvq4_workspace_bytes(const KvQ4Attention& args, int sms) {
     KvQ4Attention a = args;
+    a.sms = sms;
     plan_spans(a);
     return partial_bytes(a) + split_bytes(a) + (size_t)wanted_tiles(a) * 512 * a.head_dim * a.kv_heads;
 }
 
 cudaError_t launch_kvq4_attention(cudaStream_t stream, KvQ4Attention a) {
     if (a.rows <= 0 || a.sequences <= 0) return cudaSuccess;
+    a.sms = kvq4_sm_count();
     plan_spans(a);
     const size_t runs = partial_bytes(a), sums = runs + split_bytes(a);
     if (a.partial_bytes < sums) return cudaErrorInvalidValue;

@@ -1,5 +1,7 @@
 """Calls of the 4-bit KV cache that are refused, or sized, without a device."""
 
+import random
+
 import pytest
 
 from tests.test_kvq4_host import _args, _why
@@ -22,3 +24,18 @@ def test_sizes_beyond_32_bits_are_not_cut_to_their_low_bits():
     assert kvq4._size(-1, 50) == kvq4._size(-2 ** 32 + 5, 50) == -1
     with pytest.raises(TypeError):
         kvq4._size(None, 50)
+
+
+def test_the_workspace_is_enough_on_every_device(lib):
+    """A device plans with its own multiprocessors; more of them never need less, so that the most of the machine's devices decide."""
+    rng = random.Random(5)
+    for _ in range(400):
+        d, kv = rng.choice([64, 128, 256]), rng.choice([1, 2, 8, 64])
+        sequences, most = rng.choice([1, 3, 64, 500]), rng.choice([1, 4, 70, 2000])
+        rows, pages = sequences * rng.randint(1, most), rng.choice([1, 9, 500, 8192])
+        heads = kv * rng.choice([1, 4, 16])
+        args = _args(type=rng.randint(0, 2), head_dim=d, kv_heads=kv, q_heads=heads, sequences=sequences, rows=rows, max_rows=min(most, rows), pages_per_sequence=pages,
+                     table_stride=pages, max_keys=rng.randint(0, pages * 16), window=rng.choice([0, 0, 1000]), q_stride=heads * d, out_stride=heads * d)
+        sizes = [lib.ribn_b200_debug_kvq4_workspace(args, sms) for sms in (1, 16, 74, 132, 148, 160, 592)]
+        assert sizes == sorted(sizes), sizes
+        assert lib.ribn_b200_kvq4_workspace(args) >= sizes[4]   # a B200's, which is also what a machine without a device is told
