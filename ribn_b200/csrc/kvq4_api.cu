@@ -69,6 +69,9 @@ const char* bad_attention(const ribn_b200_kvq4_attention_args& a) {
     if ((int64_t)a.rows * a.q_heads > INT32_MAX || a.pages_per_sequence > (1 << 26) || a.max_keys > INT32_MAX - kQ4Page || a.max_rows > a.rows) {
         return "kvq4_attention: rows x q_heads, pages_per_sequence or max_keys too large, or max_rows over rows";
     }
+    // the merge's grid: columns of the page-streaming kernel in whole blocks, of which head_dim 64 and 128 have at most 64
+    const int64_t all = (int64_t)a.max_rows * (a.q_heads / a.kv_heads), columns = a.head_dim == 256 || all < 64 ? (all + 15) / 16 * 16 : 64;
+    if (columns > 0 && (int64_t)a.sequences * a.kv_heads > INT32_MAX / columns) return "kvq4_attention: too many sequences x kv_heads x rows of a sequence";
     return nullptr;
 }
 

@@ -39,3 +39,11 @@ def test_the_workspace_is_enough_on_every_device(lib):
         sizes = [lib.ribn_b200_debug_kvq4_workspace(args, sms) for sms in (1, 16, 74, 132, 148, 160, 592)]
         assert sizes == sorted(sizes), sizes
         assert lib.ribn_b200_kvq4_workspace(args) >= sizes[4]   # a B200's, which is also what a machine without a device is told
+
+
+@pytest.mark.parametrize("change", [dict(sequences=1 << 28), dict(sequences=1 << 24, kv_heads=8, q_heads=128, rows=200, max_rows=4),
+                                    dict(sequences=70000, head_dim=256, q_heads=16, kv_heads=1, rows=2000, max_rows=2000, q_stride=4096, out_stride=4096)])
+def test_more_work_than_a_grid_has_is_refused_before_anything_is_enqueued(lib, change):
+    args = _args(**change)
+    assert lib.ribn_b200_kvq4_workspace(args) == 0
+    assert lib.ribn_b200_kvq4_attention(0, None, args) == -1 and "too many" in _why(lib)
