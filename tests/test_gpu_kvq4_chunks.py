@@ -166,3 +166,120 @@ def test_scores_of_a_chunk_at_the_ends_of_the_range(kvq4, type_name, d):
 @pytest.mark.parametrize("rows,d", [(1, 128), (5, 64), (3, 256), (20, 128)])
 def test_scores_of_few_rows_at_the_ends_of_the_range(kvq4, type_name, rows, d):
     _far_ends(kvq4, *TYPES[type_name], rows, d)
+
+
+def _poisoned(cache, seen):
+    """The arena with NaN and infinite scales, and any codes, in every slot but `seen`."""
+    d = cache.bytes.shape[2] // 18
+    groups, out = d // 32, cache.bytes.clone()
+    for slot in sorted(set(range(cache.pages * 16)) - set(seen)):
+        page, j = divmod(slot, 16)
+        at = torch.tensor([16 * d + (j * groups + G) * 2 for G in range(groups)] + [17 * d + ((j // 2) * groups + G) * 4 + j % 2 * 2 for G in range(groups)], device="cuda")
+        out[page, :, at] = 0
+        out[page, :, at + 1] = torch.tensor([0x7c, 0x7e, 0xfc, 0xff], dtype=torch.uint8, device="cuda").repeat(d // 32)[:len(at)]
+    return out
+
+
+@pytest.mark.parametrize("type_name", TYPES)
+@pytest.mark.parametrize("heads,hint", [(1, 1), (1, 400), (75, 400)])
+@pytest.mark.parametrize("window", [0, 37, 200])
+def test_bytes_that_no_row_of_a_chunk_may_see_may_be_anything(kvq4, type_name, heads, hint, window):
+    dtype, unit = TYPES[type_name]
+    rng = np.random.default_rng(25)
+    keys, d, rows = 390, 64, _MANY
+    cache = _Cache(kvq4, _rows(rng, 448, heads, d, torch.float32), _rows(rng, 448, heads, d, torch.float32))
+    tables = rng.permutation(cache.pages).astype(np.int32)[None]
+    tables = np.concatenate([tables, tables[:, :2]], axis=1)   # (behind the last key: pages that are in use)
+    q = _rows(rng, rows, heads, d, dtype)
+    first = max(0, keys - rows + 1 - window) if window else 0
+    clean = _attend(kvq4, cache, q, tables, [keys], [0, rows], max_keys=hint, window=window, unit=unit, check=heads == 1 or window == 37)
+    cache.bytes = _poisoned(cache, [int(tables[0, p // 16]) * 16 + p % 16 for p in range(first, keys)])
+    assert torch.equal(_attend(kvq4, cache, q, tables, [keys], [0, rows], max_keys=hint, window=window, check=False), clean)
+
+
+@pytest.mark.parametrize("type_name", TYPES)
+@pytest.mark.parametrize("hint", [1, 41])
+def test_chunks_among_more_sequences_than_threads(kvq4, type_name, hint):
+    """Four hundred sequences of none to forty keys, every tenth with twenty rows of four heads, the others with none or one."""
+    dtype, unit = TYPES[type_name]
+    rng = np.random.default_rng(26)
+    cache = _Cache(kvq4, _rows(rng, 480, 1, 64, torch.float32), _rows(rng, 480, 1, 64, torch.float32))
+    lengths = rng.integers(0, 41, 400).tolist()
+    counts = [20 if i % 10 == 3 else i % 7 % 2 for i in range(400)]
+    assert 20 * 4 >= _MANY
+    wide = rng.integers(0, 30, (400, 5)).astype(np.int32)
+    cu = [0, *np.cumsum(counts).tolist()]
+    q = _rows(rng, cu[-1] + 5, 4, 64, dtype)
+    got = _attend(kvq4, cache, q, wide[:, :3], lengths, cu, max_keys=hint, unit=unit)
+    # the same out of a wider table
+    at = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in (lengths, cu)]
+    assert torch.equal(kvq4.attention(cache.bytes, q, torch.from_numpy(wide).cuda()[:, :3], *at, max_rows=20, max_keys=hint), got)
+
+
+@pytest.mark.parametrize("type_name", TYPES)
+@pytest.mark.parametrize("heads,d,hint", [(1, 128, 1), (1, 64, 2100), (75, 64, 2100)])
+@pytest.mark.parametrize("window", [0, 1300])
+def test_many_key_tiles_in_one_cta(kvq4, type_name, heads, d, hint, window):
+    """Seventeen key tiles behind one pair of query tiles, ten of a window, converted by the CTA, shared, or expanded; a second sequence beside it
+    whose pages come behind the first one's."""
+    dtype, unit = TYPES[type_name]
+    rng = np.random.default_rng(27)
+    lengths = [2100, 500]
+    cache = _Cache(kvq4, _rows(rng, 2640, heads, d, torch.float32, 1.5), _rows(rng, 2640, heads, d, torch.float32))
+    cu = [0, 140, 140 + _MANY] if heads == 1 else [0, _MANY, _MANY + 1]
+    q = _rows(rng, cu[-1], heads, d, dtype, 1.5)
+    _attend(kvq4, cache, q, _tables(rng, cache.pages, lengths), lengths, cu, max_keys=hint, window=window, unit=unit)
+
+
+@pytest.mark.parametrize("rows", [5, 90])
+def test_rows_beyond_the_most_stay_as_they_are(kvq4, rows):
+    """`max_rows` below what a sequence has: its later rows are left alone, the earlier ones keep their positions."""
+    rng = np.random.default_rng(28)
+    cache = _Cache(kvq4, _rows(rng, 320, 2, 64, torch.float32), _rows(rng, 320, 2, 64, torch.float32))
+    most, lengths, cu = rows - 3, [200, 90], [0, rows, rows + 2]
+    tables = _tables(rng, cache.pages, lengths)
+    q = _rows(rng, rows + 2, 4, 64, torch.float16)
+    at = [torch.from_numpy(tables).cuda(), *(torch.tensor(x, dtype=torch.int32, device="cuda") for x in (lengths, cu))]
+    out = torch.full_like(q, 5.0)
+    kvq4.attention(cache.bytes, q, *at, max_rows=most, max_keys=200, out=out)
+    want, sizes = R.attention(cache.k, cache.v, cache.pages, _host(q), tables, lengths, cu, 0, 0.125, np.zeros(q.shape))
+    assert (out[most:rows] == 5.0).all()
+    keep = [i for i in range(rows + 2) if not most <= i < rows]
+    _check(out[keep], want[keep], [x[keep] for x in sizes], torch.float16, 2.0 ** -11)
+
+
+@pytest.mark.parametrize("type_name", TYPES)
+def test_a_mixed_call_captured_and_replayed_as_its_sequences_grow(kvq4, type_name):
+    """A chunk beside single rows, captured once with a hint of 64 keys and replayed while lengths, rows per sequence and pages change, up to far more
+    keys than the hint; another call's graph with the same tensors replayed between."""
+    dtype, unit = TYPES[type_name]
+    rng = np.random.default_rng(29)
+    cache = _Cache(kvq4, _rows(rng, 1600, 2, 64, torch.float32), _rows(rng, 1600, 2, 64, torch.float32))
+    q = _rows(rng, 75, 4, 64, dtype)
+    tables, lengths, cu = (torch.zeros(s, dtype=torch.int32, device="cuda") for s in ((3, 40), (3,), (4,)))
+    outs, graphs = [torch.zeros_like(q) for _ in range(2)], [torch.cuda.CUDAGraph() for _ in range(2)]
+    call = [lambda: kvq4.attention(cache.bytes, q, tables, lengths, cu, max_rows=72, max_keys=64, out=outs[0]),
+            lambda: kvq4.attention(cache.bytes, q, tables, lengths, cu, max_rows=72, max_keys=640, window=50, out=outs[1])]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for c in call:
+            c()
+    torch.cuda.synchronize()
+    for c, g in zip(call, graphs):
+        with torch.cuda.graph(g, stream=side):
+            c()
+    for counts, sizes_of in (([72, 1, 2], [72, 9, 33]), ([1, 72, 0], [100, 500, 0]), ([1, 1, 72], [640, 1, 600]), ([30, 1, 40], [640, 640, 3]), ([0, 72, 3], [5, 71, 640])):
+        t = rng.integers(0, cache.pages, (3, 40)).astype(np.int32)
+        at = [0, *np.cumsum(counts).tolist()]
+        for to, x in ((tables, t), (lengths, np.array(sizes_of, np.int32)), (cu, np.array(at, np.int32))):
+            to.copy_(torch.from_numpy(x))
+        q.copy_(_rows(rng, 75, 4, 64, dtype))
+        before = [_host(o) for o in outs]
+        for _ in range(2):
+            for g in graphs:
+                g.replay()
+        for o, b, window in zip(outs, before, (0, 50)):
+            want, sizes = R.attention(cache.k, cache.v, cache.pages, _host(q), t, sizes_of, at, window, 0.125, b)
+            _check(o, want, sizes, dtype, unit)
+    for g in graphs:
+        g.reset()
