@@ -696,14 +696,23 @@ int wanted_tiles(const KvQ4Attention& a) {
 }
 // While query tiles leave SMs idle their keys are shared, two key tiles to a CTA at least: 16 rows behind 8,000 keys, 32 / 8 heads, 182 us
 // without.  The sums of rows x q_heads x splits are those of at most 256 rows per SM.
+// Long ranges are shared whatever the SMs: a sum in tensor memory is cut at its last bit by every product of 16 keys and comes out about 0.8 x 2^-24
+// smaller for each (F32 rows fold theirs): F16 rows behind 131,072 keys 3.9e-4 with all of them in one CTA, beside roundings of 2.3e-4, and less than
+// 1.2e-4 with 32,768.  While the sums take at most kSumsMost.  2,048 BF16 rows behind 65,536 keys, 32 / 8 heads: 2.02 ms before, 2.07
+// so; behind 131,072: 4.08 and 3.92.
+constexpr long long kLongest = 32768 / 128;
+constexpr size_t kSumsMost = 256u << 20;
+size_t sums_of(const KvQ4Attention& a) { return (size_t)a.rows * a.q_heads * (a.head_dim + 4) * sizeof(float); }
 int wanted_splits(const KvQ4Attention& a) {
     if (!has_tiles(a)) return 1;
     const long long ctas = std::max(1ll, kvq4_tile_places(a) * a.kv_heads), tiles = std::max(1ll, seen_keys(a) / 128 + 1);
-    return (int)std::max(1ll, std::min(a.sms / ctas, (tiles + 1) / 2));
+    const long long idle = std::max(1ll, std::min(a.sms / ctas, (tiles + 1) / 2));
+    const long long exact = a.type == kQ4F32 ? 1 : std::min((tiles + kLongest - 2) / kLongest, (long long)(kSumsMost / sums_of(a)));
+    return (int)std::max(idle, exact);
 }
 size_t split_bytes(const KvQ4Attention& a) {
     const int splits = wanted_splits(a);
-    return splits > 1 ? (size_t)a.rows * a.q_heads * splits * (a.head_dim + 4) * sizeof(float) : 0;
+    return splits > 1 ? splits * sums_of(a) : 0;
 }
 
 }  // namespace

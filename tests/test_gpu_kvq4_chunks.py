@@ -283,3 +283,29 @@ def test_a_mixed_call_captured_and_replayed_as_its_sequences_grow(kvq4, type_nam
             _check(o, want, sizes, dtype, unit)
     for g in graphs:
         g.reset()
+
+
+@pytest.mark.parametrize("type_name", TYPES)
+def test_a_long_range_loses_no_more_than_a_rounding(kvq4, type_name):
+    """A chunk whose query tiles fill the GPU, behind 131,072 keys.  Each product of 16 keys cuts the sum it is added to at its last bit, so a sum over n keys
+    in tensor memory comes out up to n / 16 x 2^-24 smaller: at most 2^-13 for the 32,768 keys that F16 and BF16 rows add up in one place, on top of what
+    rounds either way (probabilities, exponentials, the result), which averages out over 200,000 values.  (Not for BF16 results: the weights e^x of normal x
+    leave a standard deviation of sqrt(e / 131,072) = 4.6e-3 around 0.5, nine steps of F16 there but little more than one of BF16, 3.9e-3, whose roundings then go together.)"""
+    dtype, unit = TYPES[type_name]
+    keys, rows, heads, d = 131072, 1200, 16, 64
+    rng = torch.Generator(device="cuda").manual_seed(30)
+    cache, slots = kvq4.empty_cache(keys // 16, 1, d), torch.arange(keys, dtype=torch.int32, device="cuda")
+    k, v = (torch.randn((keys, 1, d), generator=rng, device="cuda") for _ in range(2))
+    kvq4.append(cache, k, v + 0.5, slots)
+    k, v = (x[:, 0].double() for x in kvq4.read(cache, slots, dtype=torch.float32))
+    q = torch.randn((rows, heads, d), generator=rng, device="cuda").to(dtype)
+    at = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([keys], [0, rows])]
+    got = kvq4.attention(cache, q, slots[:keys // 16][None], *at, max_rows=rows, max_keys=keys).double()
+    some = torch.arange(0, rows, 6, device="cuda")
+    x = torch.einsum("rhd,kd->rhk", q[some].double(), k) * d ** -0.5
+    x.masked_fill_(slots[None, None] > (keys - rows + some)[:, None, None], -torch.inf)
+    want = torch.einsum("rhk,kd->rhd", x.softmax(-1), v)
+    off = got[some] - want
+    less = -float((off * want).sum() / (want * want).sum())
+    assert dtype is torch.bfloat16 or abs(less) < (2.0 ** -13 if dtype is torch.float16 else 2.0 ** -19), less
+    assert float(off.norm() / want.norm()) < unit + (2.0 ** -13 if dtype is not torch.float32 else 2.0 ** -18)
