@@ -168,7 +168,7 @@ __device__ __forceinline__ Tiles tiles_before(const KvQ4Attention& a, int s, int
     int before = 0;
     for (int i = lane; i < s; i += 32) {
         int tile0, low, high;
-        before += tiles_of(a, i, tile0, low, high);
+        before = min(before + tiles_of(a, i, tile0, low, high), 1 << 20);   // (more than any scratch has; 32 such sums fit in the word)
     }
     Tiles r;
     r.first = __reduce_add_sync(0xffffffffu, before);
