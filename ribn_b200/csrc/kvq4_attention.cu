@@ -116,7 +116,7 @@ __device__ __forceinline__ Sequence sequence_of(const KvQ4Attention& a, int s) {
 // Pages per CTA of a list of `total`: whole rounds of the four warps
 __device__ __forceinline__ long long share_of(const KvQ4Attention& a, long long total) {
     const long long even = (total + a.grid - 1) / a.grid;
-    return (max(even, (long long)a.least_pages) + kWarps - 1) / kWarps * kWarps;
+    return (max(even, (long long)kWarps) + kWarps - 1) / kWarps * kWarps;
 }
 // One item's columns
 struct Block {
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 && NT == 1 ? 3 : 2) kvq
     const long long share = share_of(a, total);
     long long at = blockIdx.x * share;
     const long long stop = min(total, at + share);
-    if (blockIdx.x == 0 && a.may_cut) {   // for the merge
+    if (blockIdx.x == 0 && a.grid > 1) {   // for the merge: an item may have runs in several CTAs
         long long x = before;
         for (int i = s0; i < s1; ++i) { a.prefix[i] = x; x += sequence_of(a, i).weight(a.kv_heads); }
         if (threadIdx.x == 0) a.prefix[a.sequences] = total;
@@ -619,9 +619,7 @@ void plan_spans(KvQ4Attention& a) {
     const long long keys = a.window > 0 ? std::min<long long>(a.max_keys, (long long)a.window + a.max_rows + kQ4Page) : a.max_keys;
     const long long pages = std::max(1ll, (keys + kQ4Page - 1) / kQ4Page), items = (long long)a.sequences * a.kv_heads * a.col_blocks;
     const long long resident = (long long)a.sms * (a.head_dim <= 128 && a.span_cols == 8 ? 3 : 2);   // as their launch bounds say
-    a.least_pages = kWarps;
-    a.grid = (int)std::max(1ll, std::min(resident, (items * pages + a.least_pages - 1) / a.least_pages));
-    a.may_cut = a.grid > 1;   // an item may have runs in several CTAs
+    a.grid = (int)std::max(1ll, std::min(resident, (items * pages + kWarps - 1) / kWarps));
 }
 
 template <typename Kernel>
@@ -662,7 +660,7 @@ cudaError_t launch_hd(cudaStream_t stream, const KvQ4Attention& a) {
     const bool pair = a.type == kQ4F32;
     cudaError_t e = a.span_cols == 8 ? (pair ? launch_spans<HD, 1, true>(stream, a) : launch_spans<HD, 1, false>(stream, a))
                                      : (pair ? launch_spans<HD, WIDE, true>(stream, a) : launch_spans<HD, WIDE, false>(stream, a));
-    if (e == cudaSuccess && a.may_cut) e = launch(stream, kvq4_merge_kernel<HD>, (long long)a.sequences * a.kv_heads * a.col_blocks * a.merge_cols, 0, a);
+    if (e == cudaSuccess && a.grid > 1) e = launch(stream, kvq4_merge_kernel<HD>, (long long)a.sequences * a.kv_heads * a.col_blocks * a.merge_cols, 0, a);
     return e;
 }
 
@@ -683,7 +681,7 @@ namespace {
 constexpr size_t kScratchMost = 512u << 20;
 size_t prefix_bytes(const KvQ4Attention& a) { return ((size_t)a.sequences + 1) * sizeof(long long); }
 size_t partial_bytes(const KvQ4Attention& a) {
-    const size_t n = a.may_cut ? prefix_bytes(a) + (size_t)a.grid * 2 * a.span_cols * (a.head_dim + 2) * sizeof(float) : 0;
+    const size_t n = a.grid > 1 ? prefix_bytes(a) + (size_t)a.grid * 2 * a.span_cols * (a.head_dim + 2) * sizeof(float) : 0;
     return (n + 255) / 256 * 256;
 }
 bool has_tiles(const KvQ4Attention& a) { return (long long)std::min(a.max_rows, a.rows) * (a.q_heads / a.kv_heads) > a.tile_above; }

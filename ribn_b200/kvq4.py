@@ -60,7 +60,7 @@ def _ints(name: str, x: torch.Tensor, shape: tuple, device: int):
     return x.data_ptr()
 
 
-_MOST = 2 ** 31 - 1
+_MOST, _MOST_KEYS = 2 ** 31 - 1, 2 ** 31 - 1 - PAGE_TOKENS
 
 
 def _size(x: int, most: int) -> int:
@@ -130,9 +130,11 @@ def attention(cache: torch.Tensor, q: torch.Tensor, page_tables: torch.Tensor, l
     if out is None:
         out = torch.zeros((rows, q_heads, head_dim), dtype=q.dtype, device=q.device)
     out_stride = _rows("out", out, q_heads, head_dim, device, rows, q.dtype)
+    if not (0 <= max_rows <= rows and 0 <= max_keys <= _MOST_KEYS and 0 <= window <= _MOST):   # (one test in the common case, 1 us less)
+        max_rows, max_keys, window = _size(max_rows, rows), _size(max_keys, _MOST_KEYS), _size(window, _MOST)
     args = KvQ4AttentionArgs(cache.data_ptr(), pages, q.data_ptr(), out.data_ptr(), tables, at_lengths, at_rows, None, 0, q_stride, out_stride,
                              page_tables.stride(0), _TYPES[q.dtype], q_heads, kv_heads, head_dim, width, sequences, rows,
-                             _size(max_rows, rows), _size(max_keys, _MOST - PAGE_TOKENS), _size(window, _MOST), scale or 0.0, 0)
+                             max_rows, max_keys, window, scale or 0.0, 0)
     library = lib()
     need = library.ribn_b200_kvq4_workspace(args)
     if need:
