@@ -309,3 +309,24 @@ def test_a_long_range_loses_no_more_than_a_rounding(kvq4, type_name):
     less = -float((off * want).sum() / (want * want).sum())
     assert dtype is torch.bfloat16 or abs(less) < (2.0 ** -13 if dtype is torch.float16 else 2.0 ** -19), less
     assert float(off.norm() / want.norm()) < unit + (2.0 ** -13 if dtype is not torch.float32 else 2.0 ** -18)
+
+
+@pytest.mark.parametrize("type_name", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hint", [1, 12000])
+def test_many_small_probabilities_behind_a_large_one(kvq4, type_name, d, hint):
+    """Three keys have e^17.5 = 2^25.2 times the probability of each of 12,000 others: added one by one to a sum in F32 these would all be lost, and
+    together they are 1e-4 of it.  (Scores are exact: one dimension, of a few bits.)"""
+    dtype, unit = TYPES[type_name]
+    rng = np.random.default_rng(33)
+    keys = 12000
+    k = np.zeros((keys, 1, d), np.float32)
+    k[[3, 200, 5000], 0, 5] = 17.5
+    v = rng.normal(0.5, 0.5, (keys, 1, d)).astype(np.float32)
+    cache = _Cache(kvq4, torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda())
+    q = np.zeros((_MANY, 2, d), np.float32)
+    q[:, :, 5] = rng.choice([4.0, 3.75, 0.0, -4.0], (_MANY, 2))
+    tables = np.arange(cache.pages, dtype=np.int32)[None]
+    window = keys - 2000   # (the first rows see the key at 5,000 only, whatever the last ones see)
+    for w in (0, window):
+        _attend(kvq4, cache, torch.from_numpy(q).to(dtype).cuda(), tables, [keys], [0, _MANY], max_keys=hint, window=w, scale=0.25, unit=unit)
