@@ -136,6 +136,11 @@ __device__ __forceinline__ Block block_of(const KvQ4Attention& a, const Sequence
 }
 
 constexpr int kRing = 4;   // page records per warp: one read, three on their way
+// F32 rows: a thread's sums move to shared memory after so many pages.  In one place, thousands of keys of 2^-25 of the largest fell below the sums'
+// last bits (one row, 60,000 keys of which three have all but 5e-4, one CTA: 3.8e-5 off, so less than 4e-6).
+constexpr int kKept = 32;
+template <int HD, int NT, bool PAIR>
+constexpr size_t kSpanSmem = (size_t)kWarps * kRing * q4_record(HD) + (PAIR ? kWarps * 32 * (2 + HD / 4) * NT * sizeof(float) : 0);
 
 // NT: column tiles of 8.  PAIR: F32 queries.
 template <int HD, int NT, bool PAIR>
@@ -321,9 +326,26 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 && NT == 1 ? 3 : 2) kvq
         m[nt][0] = m[nt][1] = -INFINITY;
         l[nt][0] = l[nt][1] = 0.0f;
     }
+    // PAIR, of each column tile: where l and o are kept, kWarps * 32 floats apart
+    const bool keeps = PAIR && mine > kKept;
+    float* const kept = reinterpret_cast<float*>(smem + kWarps * RING * RECORD) + threadIdx.x;
+    constexpr int KEPT = (2 + 8 * NG) * kWarps * 32;
+    auto keep = [&](bool first) {   // the sums so far, and from zero on
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int u = 0; u < 2 + 8 * NG; ++u) {
+                float& x = u < 2 ? l[nt][u & 1] : o[nt][(u - 2) >> 2 & (2 * NG - 1)][(u - 2) & 3];
+                float* const to = kept + nt * KEPT + u * kWarps * 32;
+                *to = first ? x : *to + x;
+                x = 0.0f;
+            }
+        }
+    };
 
     for (int i = 0; i < mine; ++i) {
         issue(i + RING - 1);
+        if (PAIR && i > 0 && i % kKept == 0) keep(i == kKept);
         asm volatile("cp.async.wait_group %0;" ::"n"(RING - 1) : "memory");
         __syncwarp();
         if (!((good >> (i & 31)) & 1u)) continue;
@@ -417,6 +439,10 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 && NT == 1 ? 3 : 2) kvq
                 }
 #pragma unroll
                 for (int mt = 0; mt < 2 * NG; ++mt) { o[nt][mt][0] *= f[0]; o[nt][mt][1] *= f[1]; o[nt][mt][2] *= f[0]; o[nt][mt][3] *= f[1]; }
+                if (PAIR && i >= kKept) {
+#pragma unroll 4
+                    for (int u = 0; u < 2 + 8 * NG; ++u) kept[nt * KEPT + u * kWarps * 32] *= f[u & 1];
+                }
             }
         }
         uint32_t ph[NT][2], pl[PAIR ? NT : 1][2];
@@ -477,6 +503,13 @@ __global__ void __launch_bounds__(kWarps * 32, HD <= 128 && NT == 1 ? 3 : 2) kvq
             }
         }
         __syncwarp();   // every lane has read the slot before the next copies land in it
+    }
+    if (keeps) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int u = 0; u < 2 + 8 * NG; ++u) (u < 2 ? l[nt][u & 1] : o[nt][(u - 2) >> 2 & (2 * NG - 1)][(u - 2) & 3]) += kept[nt * KEPT + u * kWarps * 32];
+        }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncwarp();
@@ -640,7 +673,7 @@ cudaError_t launch(cudaStream_t stream, Kernel kernel, long long grid, size_t sm
 
 template <int HD, int NT, bool PAIR>
 cudaError_t launch_spans(cudaStream_t stream, const KvQ4Attention& a) {
-    constexpr size_t smem = (size_t)kWarps * kRing * q4_record(HD);
+    constexpr size_t smem = kSpanSmem<HD, NT, PAIR>;
     static bool configured[kMaxDevices] = {false};   // function attributes are per device
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);

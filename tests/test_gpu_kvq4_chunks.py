@@ -330,3 +330,24 @@ def test_many_small_probabilities_behind_a_large_one(kvq4, type_name, d, hint):
     window = keys - 2000   # (the first rows see the key at 5,000 only, whatever the last ones see)
     for w in (0, window):
         _attend(kvq4, cache, torch.from_numpy(q).to(dtype).cuda(), tables, [keys], [0, _MANY], max_keys=hint, window=w, scale=0.25, unit=unit)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("heads,rows", [(4, 1), (4, 4)])
+def test_many_small_probabilities_of_single_rows(kvq4, d, heads, rows):
+    """The same for F32 rows of the other kernel, whose warps have 15,000 keys each (a hint of one key: one CTA for all).  Here scores are exact, so that what
+    may be off is what probabilities as pairs and the sums' order leave (2^-19), and half a step of 2^-24 for each small probability, of the sum of three of 2^7."""
+    rng = np.random.default_rng(34)
+    keys = 60000
+    k = np.zeros((keys, 1, d), np.float32)
+    k[[3, 200, 5000], 0, 5] = 17.5
+    v = rng.normal(0.5, 0.5, (keys, 1, d)).astype(np.float32)
+    cache = _Cache(kvq4, torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda())
+    q = np.zeros((rows, heads, d), np.float32)
+    q[:, :, 5] = 4.0
+    q = torch.from_numpy(q).cuda()
+    tables = np.arange(cache.pages, dtype=np.int32)[None]
+    for hint in (1, keys):
+        got = _attend(kvq4, cache, q, tables, [keys], [0, rows], max_keys=hint, scale=0.25, check=False)
+        want, (weight, extent, _) = R.attention(cache.k, cache.v, cache.pages, _host(q), tables, [keys], [0, rows], 0, 0.25, np.zeros(q.shape))
+        assert np.all(np.abs(_host(got) - want) <= weight * 2.0 ** -19 + extent * 2.0 ** -25 / (3 * 2.0 ** 7)), hint
