@@ -4,7 +4,8 @@
 // with softmax warps of its own, so that one tile's products run while the other's probabilities are formed.  Per 128 keys:
 //   S = Q K^T   A = the queries as binary16 in shared memory, scaled by a power of two per row, B = K;
 //   P           two threads own a row, 64 keys each: softmax in base 2 against a reference that moves only when a score passes it by
-//               2^8, P (held 2^7 times, so that small ones stay normal numbers) as binary16 over S in tensor memory;
+//               2^8, P (held 2^7 times, so that small ones stay normal numbers) as binary16 over S in tensor memory, divided at the end by
+//               the sum of the rounded ones, so that a row's weights add up to one (1.1 % of the time; a row of one key has its value);
 //   O += P V    A = P from tensor memory, B = V^T.
 // K and V^T come as operands: from memory, where kvq4_expand_kernel has left them, once for all query rows of a call, or, where the
 // call has no room for that, from seven warps that turn page records into them.  A nibble under the exponent of 64 is 64 + code; one
@@ -743,10 +744,11 @@ __global__ void __launch_bounds__(Tile<HD, PAIR>::THREADS, 1) kvq4_tile_kernel(c
                         for (int u = 0; u < 16; ++u) {
                             const float2 y = __ffma2_rn(make_float2(s[2 * u], s[2 * u + 1]), make_float2(times, times), make_float2(shift, shift));
                             const float2 p = (u * kPolynomial) % 16 < kPolynomial ? exp2_pair(y) : make_float2(exp2_approx(y.x), exp2_approx(y.y));
-                            const float2 lp = __fadd2_rn(make_float2(l0, l1), p);
+                            const __half2 rounded = __floats2half2_rn(p.x, p.y);   // what the products take
+                            const float2 lp = __fadd2_rn(make_float2(l0, l1), __half22float2(rounded));
                             l0 = lp.x;
                             l1 = lp.y;
-                            hi[u] = as_bits(__floats2half2_rn(p.x, p.y));
+                            hi[u] = as_bits(rounded);
                         }
                         if (!pair_any(mx > m + kSlack)) break;
                         tmem_wait_st();   // what is read back below may have been stored in this tile: earlier probabilities, sums of an earlier move

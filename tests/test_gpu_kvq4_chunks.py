@@ -351,3 +351,22 @@ def test_many_small_probabilities_of_single_rows(kvq4, d, heads, rows):
         got = _attend(kvq4, cache, q, tables, [keys], [0, rows], max_keys=hint, scale=0.25, check=False)
         want, (weight, extent, _) = R.attention(cache.k, cache.v, cache.pages, _host(q), tables, [keys], [0, rows], 0, 0.25, np.zeros(q.shape))
         assert np.all(np.abs(_host(got) - want) <= weight * 2.0 ** -19 + extent * 2.0 ** -25 / (3 * 2.0 ** 7)), hint
+
+
+@pytest.mark.parametrize("type_name", TYPES)
+@pytest.mark.parametrize("rows,hint", [(_MANY, 1), (_MANY, 4000), (3, 4000)])
+def test_a_row_of_one_key_has_its_value(kvq4, type_name, rows, hint):
+    """However its probability is rounded: F16 rows have the cached value exactly, BF16 ones as it rounds, F32 ones but for the probability's rounding
+    as a pair (2^-22) and those of the sum, the quotient and the result (2^-24 each)."""
+    dtype, unit = TYPES[type_name]
+    rng = np.random.default_rng(35)
+    cache = _Cache(kvq4, _rows(rng, 200, 2, 128, torch.float32), _rows(rng, 200, 2, 128, torch.float32))
+    tables = rng.permutation(cache.pages).astype(np.int32)[None]
+    q = _rows(rng, rows, 4, 128, dtype, 2.0)
+    got = _host(_attend(kvq4, cache, q, tables, [190], [0, rows], max_keys=hint, window=1, unit=unit))
+    at = np.array([tables[0, p // 16] * 16 + p % 16 for p in range(190 - rows, 190)])
+    want = cache.v[at][:, [0, 0, 1, 1]]
+    if dtype is torch.float16:
+        assert np.array_equal(got, want)
+    else:
+        assert np.all(np.abs(got - want) <= np.abs(want) * (unit * (1 + 2.0 ** -14) if dtype is torch.bfloat16 else 2.0 ** -21))
