@@ -483,7 +483,10 @@ RIBN_B200_API int ribn_b200_kvq4_read(int32_t device, void* stream, const void* 
  * the pages page_tables[s * table_stride ..]: row i of n is at position lengths[s] - n + i and sees the keys up to its own, with
  * window > 0 the last `window` of those.  A row that sees no key (its position is negative) gets zeros; rows of q that no
  * sequence has are left alone in `out`; a page number outside of the arena hides its keys.  `max_rows` bounds the rows of
- * a sequence (later ones are left alone); `max_keys` sets how the work is split, results are right for any.  `scale` 0 is
+ * a sequence (later ones are left alone); `max_keys` sets how the work is split, results are right for any (but see below).  F32 rows'
+ * probabilities are held as pairs of binary16, F16 and BF16 ones as one, and their sums are cut at the last bit for every 16 keys that lie in one
+ * place (at most 32,768, where max_keys is the longest length): F16 results are up to 1.3 times as far from exact ones as their own rounding.
+ * A query that is not finite makes its row NaN where it sees a key.  `scale` 0 is
  * 1 / sqrt(head_dim).  `q_stride`, `out_stride`: values from one row to the next; `out` does not overlap `q`.  At most 2^26 pages
  * per sequence.  `workspace` (16-byte aligned, what ribn_b200_kvq4_workspace asks for; the part that it asks for operands of
  * sequences with many rows may be missing, which is slower) is scratch of this call: calls that may overlap on the GPU, or graphs that may replay

@@ -21,7 +21,7 @@
 //
 // What bounds it: issuing.  A page takes a warp about 330 instructions, 96 of them on the logic pipe, which starts one every other
 // clock, and three CTAs of four warps per SM issue two of three clocks: sixteen BF16 sequences of up to 32,768 keys, 32 / 8 heads, 395 MB,
-// 100 us, 61 % of the copy bandwidth.  Short calls are a chain of memory's latencies: where the CTA's run begins, queries and page
+// 97 us, 62 % of the copy bandwidth.  Short calls are a chain of memory's latencies: where the CTA's run begins, queries and page
 // numbers, pages, and the merge's; one sequence of 1,024 keys takes 14 us with its append.  Tried: a grid of (span, item) instead of the
 // list 142 us for the sixteen, four CTAs per SM with 48 bytes of spills 103; for up to 16 columns three CTAs instead of two, 290 bytes of
 // spills, 175 against 166 us (40 sequences of four rows, windows of 4,096 keys), and blocks of 8 columns 189.
@@ -644,7 +644,8 @@ bool aligned16(const void* p, long long stride, int size) { return (reinterpret_
 void plan_spans(KvQ4Attention& a) {
     const int group = a.q_heads / a.kv_heads;
     // More columns take the tensor-memory kernel: eight BF16 sequences of 2,000 keys with 64 columns 55 us here and 80 there, with 128 91 and
-    // 66.  (Heads of 256 have no such kernel: two tiles' sums would fill tensor memory.)
+    // 66.  (Heads of 256 have no such kernel: two tiles' sums would take all of tensor memory;
+    // one tile a CTA would fit and was not built.)
     a.tile_above = a.head_dim == 256 ? 0x7fffffff : 64;
     const int cols = (int)std::min<long long>((long long)std::min(a.max_rows, a.rows) * group, a.tile_above);
     // 16 columns share a page's conversion; with heads of 256 their sums do not fit in the registers (1,080 bytes of spills)

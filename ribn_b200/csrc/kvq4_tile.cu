@@ -19,11 +19,11 @@
 //
 // What bounds it: a tile's chain.  Its products take 1,024 clocks, its scores 1,300 to 1,600 to become probabilities (exponentials: 16 a
 // clock per SM, a quarter of them moved to the multiply-add pipe), and handing over costs about 700 each time, while the other tile's
-// products fill 1,024 of that.  2,048 BF16 rows behind 14,336 keys, 32 / 8 heads: 520 us with 16 us of expansion before it, 891 TFLOP/s
-// of the whole call (256 CTAs on 148 SMs: the second turn fills 73 % of them).  Tried: conversion by seven warps beside it 585; one
+// products fill 1,024 of that.  2,048 BF16 rows behind 14,336 keys, 32 / 8 heads: 555 us in a replayed graph with their append, 16 us of
+// expansion and cold inputs, 928 TFLOP/s (256 CTAs on 148 SMs: the second turn fills 73 % of them).  Tried, of the kernel when it took 520: conversion by seven warps beside it 585; one
 // thread per row 545 (its instructions wait for one another); one vote per 128 scores, with spills, 720; a warp per tile for the
 // products 565 (both tiles' products then run at the same time, and both softmaxes); no exponentials by the polynomial 553.
-// Short chunks are latencies and instructions fetched for the first time: 777 F32 rows of 16 / 8 heads 53 us with append and merges.
+// Short chunks are latencies and instructions fetched for the first time: 777 F32 rows of 16 / 8 heads 51 us with append and merges.
 #include <cuda_fp16.h>
 #include <math.h>
 

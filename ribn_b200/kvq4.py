@@ -75,7 +75,7 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda de
 def append(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """Quantises rows k, v [rows][kv_heads][head_dim] into the arena at slots[row] = page * 16 + token.  A row with a slot outside
     of the arena (-1: padding) is not written.  The slots of one call are distinct.  NaN counts as zero, magnitudes over 7,168
-    saturate."""
+    saturate.  A cache holds bytes: no gradient passes through it."""
     pages, kv_heads, head_dim, device = _arena(cache)
     k_stride = _rows("k", k, kv_heads, head_dim, device)
     rows = k.shape[0]
@@ -109,8 +109,12 @@ def attention(cache: torch.Tensor, q: torch.Tensor, page_tables: torch.Tensor, l
     rows of sequence s, which has lengths[s] keys (these rows' own, already appended, among them) in the pages page_tables[s].
     Row i of n sits at position lengths[s] - n + i and sees the keys up to its own, with window > 0 the last `window` of those.
 
+    Probabilities of float32 rows are held as pairs of binary16, of float16 and bfloat16 ones as one: float16 results are up to 1.3 times as far
+    from exact ones as their own rounding.  A query that is not finite makes its row NaN where it sees a key.
+
     Rows that see no key get zeros, rows behind the last sequence stay as they are in `out` (zeros in a new one).  `max_rows` is
-    the most rows of a sequence; `max_keys`, about the longest length, decides how the work is split and no result.
+    the most rows of a sequence; `max_keys`, about the longest length, decides how the work is split and no result but for its last bits (below
+    a true length of more than 32,768, sums of float16 rows lose up to 2^-24 for every 16 keys).  `out` does not overlap `q`.
     `scale` defaults to head_dim ** -0.5.  There is no backward pass: a `q` or `out` that requires a gradient is refused while gradients
     are recorded.  Returns `out`, of q's type."""
     pages, kv_heads, head_dim, device = _arena(cache)
